@@ -58,9 +58,13 @@ SOURCES = [
     "csrc/hip/attention_wave_d32_o1.hip",
     "csrc/hip/attention_wave_d32_o0.hip",
     "csrc/hip/attention_wave.hip",
+    *(f"csrc/hip/paged_attention_d{d}.hip" for d in (256, 192, 128, 96, 64, 32)),
+    "csrc/hip/paged_merge.hip",
+    "csrc/hip/paged_rope.hip",
     "csrc/hip/codec_kernels.hip",
     "csrc/hip/attention_kernels.hip",
     "csrc/host/kvexp_hip_api.cpp",
+    "csrc/host/kvexp_paged_api.cpp",
 ]
 CXX_SOURCES = ["csrc/host/kvexp_cpp_api.cpp"]
 HEADERS = [
@@ -69,6 +73,11 @@ HEADERS = [
     "csrc/hip/kvexp_device.h",
     "csrc/hip/kvexp_expf.h",
     "csrc/hip/kvexp_types.h",
+    "csrc/hip/paged_attention.h",
+    "csrc/hip/paged_attention_launch.h",
+    "csrc/hip/paged_device.h",
+    "csrc/hip/paged_types.h",
+    "csrc/host/api_common.hpp",
     "csrc/host/host_walk.hpp",
     "../include/kvexp_hip.h",
     "../include/kvexp/attention.hpp",

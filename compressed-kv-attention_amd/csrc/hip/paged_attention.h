@@ -1,0 +1,743 @@
+// Attention over a paged cache and over a prefix that a batch shares
+// (templates; instantiated per head_dim in paged_attention_d*.hip).
+//
+// A query row r of a (sequence, KV head) sees the tokens [0, limit_r). With
+// s_j = scale2 * (q . k_j) (scale2 = scale log2 e), m the running maximum and
+// p_j = 2^(s_j - m), a pass over the tokens keeps m, l = sum p_j and
+// acc = sum p_j v_j, and turns acc and l by 2^(m_old - m) when m moves. A
+// token range per workgroup; the states of a row's ranges are joined by
+// paged_merge_kernel: M = max m_i, out = sum 2^(m_i - M) acc_i / sum 2^(m_i - M) l_i,
+// lse = (M + log2 l) ln 2. A row that sees nothing gives 0 and -inf.
+//
+// Both kernels form S^T = K Q^T and O^T = V^T P^T on the matrix cores, so that
+// a query row is a column of both products: a lane holds its row's scores, its
+// maximum, and its outputs, and P goes from the first product's result to the
+// second's operand without a move (the tokens of a lane's results are taken as
+// the tokens of its operand; V is read in the same order).
+#pragma once
+
+#include "paged_device.h"
+
+#include <hip/hip_fp16.h>
+
+namespace kvexp_dev {
+namespace paged {
+
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4a __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int kPagedThreads = 256;
+constexpr int kPagedWaves = 4;
+
+template <bool HALF>
+__device__ __forceinline__ f32x4 mfma16(const u32x4a &a, const u32x4a &b, const f32x4 &c) {
+    if constexpr (HALF)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <bool HALF>
+__device__ __forceinline__ f32x16 mfma32(const u32x4a &a, const u32x4a &b, const f32x16 &c) {
+    if constexpr (HALF)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Two floats to 16 bits each, rounded to nearest, x in the low half.
+template <bool HALF>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    if constexpr (HALF) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, h2{_Float16(x), _Float16(y)});
+    } else {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, b2{__bf16(x), __bf16(y)});
+    }
+}
+template <bool HALF>
+__device__ __forceinline__ float low_f32(uint32_t w) {
+    if constexpr (HALF) return __half2float(__ushort_as_half(uint16_t(w & 0xFFFFu)));
+    else return bits_f32(w << 16);
+}
+template <bool HALF>
+__device__ __forceinline__ float high_f32(uint32_t w) {
+    if constexpr (HALF) return __half2float(__ushort_as_half(uint16_t(w >> 16)));
+    else return bits_f32(w & 0xFFFF0000u);
+}
+template <bool HALF>
+__device__ __forceinline__ uint16_t to_16(float x) {
+    return uint16_t(pack2<HALF>(x, 0.0f) & 0xFFFFu);
+}
+
+__device__ __forceinline__ float exp2_f32(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Whether either half of a pair of values is an infinity or a NaN.
+template <bool HALF>
+__device__ __forceinline__ bool wild2(uint32_t w) {
+    constexpr uint32_t E = HALF ? 0x7C00u : 0x7F80u;
+    return (w & E) == E || (w & (E << 16)) == (E << 16);
+}
+
+// The rows of a workgroup: which query rows, which tokens they see.
+struct Rows {
+    int seq, head;
+    int first;  // first token row of the sequence (or of the call, shared)
+    int n;      // its new tokens
+    int len;    // tokens that may be seen
+    int count;  // rows: n * group
+    int t0, t1; // the split's tokens (t1: past the last token any row of the tile sees)
+    int split_len;
+    bool used;  // the split holds tokens of the sequence
+};
+
+// Tokens per split: at least min_split (a multiple of kSplitStep), and n_splits
+// of them reach len.
+constexpr int kSplitStep = 64;
+__device__ __forceinline__ int split_tokens(int len, int n_splits, int min_split) {
+    const int even = len / n_splits + (len % n_splits != 0);
+    return max(min_split, (even + kSplitStep - 1) / kSplitStep * kSplitStep);
+}
+
+// Raises the call's length errors once per sequence.
+__device__ __forceinline__ void find_rows(const PagedAttnArgs &a, int seq, int split, int tile, int tile_rows,
+                                          Rows &r) {
+    r.seq = seq;
+    if (a.shared) {
+        r.first = 0;
+        r.n = a.batch.n_tokens;
+        r.len = a.len;
+    } else {
+        int n;
+        new_rows(a.batch, seq, r.first, n);
+        r.n = min(n, a.batch.max_new);
+        const int held = a.batch.lens[seq];
+        const int64_t most = int64_t(a.batch.table_width) * a.pool.page_tokens;
+        r.len = int(min(int64_t(max(held, 0)), most));
+        if ((n != r.n || held > r.len) && split == 0 && tile == 0 && threadIdx.x == 0) atomicOr(a.status, kStLength);
+    }
+    r.count = r.n * a.group;
+    r.split_len = split_tokens(r.len, a.n_splits, a.min_split);
+    r.t0 = min(int64_t(split) * r.split_len, int64_t(r.len));
+    r.used = split == 0 || r.t0 < r.len;
+    const int last = min((tile + 1) * tile_rows, r.count) - 1; // last row of the tile
+    int seen = r.len;
+    if (!a.shared) seen = max(0, min(r.len, r.len - r.n + last / a.group + 1));
+    r.t1 = min(r.t0 + r.split_len, seen);
+}
+
+// Tokens that row `row` sees (0 past the rows).
+__device__ __forceinline__ int row_limit(const PagedAttnArgs &a, const Rows &r, int row) {
+    if (row >= r.count) return 0;
+    if (a.shared) return r.len;
+    return max(0, min(r.len, r.len - r.n + row / a.group + 1));
+}
+
+// Row `row`'s token row in the call's tensors.
+__device__ __forceinline__ int row_token(const PagedAttnArgs &a, const Rows &r, int row) {
+    return r.first + row / a.group;
+}
+
+__device__ __forceinline__ int page_at(const PagedAttnArgs &a, const int32_t *table, int tok, int &in_page) {
+    const int col = page_of(a.pool, tok);
+    in_page = tok - col * a.pool.page_tokens;
+    int page = table[col];
+    if (uint32_t(page) >= uint32_t(a.pool.n_pages)) {
+        atomicOr(a.status, kStPage);
+        page = 0;
+    }
+    return page;
+}
+
+// The state slot of a row and split.
+__device__ __forceinline__ int64_t state_slot(const PagedAttnArgs &a, const Rows &r, int head, int split, int row) {
+    return ((int64_t(r.seq) * a.n_kv + head) * a.n_splits + split) * a.max_rows + row;
+}
+
+// The sums of a row that saw l 0 are nothing: its output is 0.
+__device__ __forceinline__ float finish(float acc, float l) { return l == 0.0f ? 0.0f : acc / l; }
+__device__ __forceinline__ float log_sum(float m, float l) {
+    return l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * 0.69314718055994530942f;
+}
+
+// One channel of a row's state, to its slot or, where the call has one split,
+// to the output.
+template <bool HALF>
+__device__ __forceinline__ void write_state(const PagedAttnArgs &a, const Rows &r, int head, int split, int row, int d,
+                                            float m, float l, float acc) {
+    if (a.direct) {
+        const int64_t tok = row_token(a, r, row);
+        const int hq = head * a.group + row % a.group;
+        a.out.p[tok * a.out.token + int64_t(hq) * a.out.head + d] = to_16<HALF>(finish(acc, l));
+        if (d == 0 && a.lse != nullptr) a.lse[tok * (a.n_kv * a.group) + hq] = log_sum(m, l);
+        return;
+    }
+    const int64_t slot = state_slot(a, r, head, split, row);
+    a.acc[slot * a.dim + d] = acc;
+    if (d == 0) {
+        a.ml[2 * slot] = m;
+        a.ml[2 * slot + 1] = l;
+    }
+}
+
+// --------------------------------------------------------------- few rows --
+// At most 16 query rows per workgroup (a decode step's queries of one KV
+// head): 16 x 16 x 32 products, one per 16 tokens and 32 channels. K and V go
+// from memory to registers, each once: lane (c, g) of a product takes 8
+// channels of token c of K, and of V all its channels (DP / 16 of them) of
+// the 8 tokens 4 g .. 4 g + 3 and 16 + 4 g .., which its own P values belong
+// to; a few byte permutes pair the tokens. The four waves take the split's
+// 32-token tiles in turn and join their states at the end in LDS.
+template <int DP>
+struct Few {
+    static constexpr int KS = DP / 32;   // steps of 32 channels
+    static constexpr int C = DP / 16;    // channels of V per lane
+    static constexpr int VW = C / 2;     // their dwords
+    static constexpr int JC = DP > 192 ? DP / 2 : DP; // channels joined at a time (LDS below 64 KiB)
+    static constexpr int Row = JC + 4;   // floats per row of the joint state
+};
+
+// N dwords at a 4-byte aligned address.
+template <int N>
+__device__ __forceinline__ void load_words(const uint16_t *p, uint32_t *w) {
+    const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
+    typedef uint32_t x4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef uint32_t x2 __attribute__((ext_vector_type(2), aligned(4)));
+    int i = 0;
+#pragma unroll
+    for (; i + 4 <= N; i += 4) {
+        const x4 v = *reinterpret_cast<const x4 *>(q + i);
+        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+    }
+    if (N - i >= 2) {
+        const x2 v = *reinterpret_cast<const x2 *>(q + i);
+        w[i] = v.x, w[i + 1] = v.y;
+        i += 2;
+    }
+    if (N - i == 1) w[i] = q[i];
+}
+
+template <int DP>
+struct FewTile {
+    u32x4a k[2][Few<DP>::KS];
+    uint32_t v[8][Few<DP>::VW];
+};
+
+// Requests the 32 tokens from `tok` (tokens past t1 read token t1 - 1 again).
+template <int DP>
+__device__ __forceinline__ void few_load(const PagedAttnArgs &a, const Rows &r, const int32_t *table,
+                                         const uint16_t *kh, const uint16_t *vh, int tok, int vc,
+                                         FewTile<DP> &f) {
+    using F = Few<DP>;
+    const int lane = lane_id(), c = lane & 15, g = lane >> 4;
+    const int last = r.t1 - 1;
+    int in_page;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int page = page_at(a, table, min(tok + 16 * j + c, last), in_page);
+        const uint16_t *row = kh + int64_t(page) * a.pool.k_page + int64_t(in_page) * a.pool.k_token;
+#pragma unroll
+        for (int i = 0; i < F::KS; ++i) {
+            const int ch = 32 * i + 8 * g;
+            if (DP % 64 == 0 && a.dim == DP) f.k[j][i] = *reinterpret_cast<const u32x4a *>(row + ch);
+            else f.k[j][i] = ch < a.dim ? *reinterpret_cast<const u32x4a *>(row + ch) : u32x4a{0, 0, 0, 0};
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+        const int page = page_at(a, table, min(tok + 4 * g + (n & 3) + 16 * (n >> 2), last), in_page);
+        const uint16_t *row = vh + int64_t(page) * a.pool.v_page + int64_t(in_page) * a.pool.v_token;
+        load_words<F::VW>(row + vc, f.v[n]);
+    }
+}
+
+// V of channel jj of the lane for its 8 tokens, as a product's operand.
+template <int DP>
+__device__ __forceinline__ u32x4a few_v(const FewTile<DP> &f, int jj) {
+    u32x4a x;
+    const uint32_t sel = jj & 1 ? 0x07060302u : 0x05040100u;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) x[n] = __builtin_amdgcn_perm(f.v[2 * n + 1][jj >> 1], f.v[2 * n][jj >> 1], sel);
+    return x;
+}
+
+template <int DP, bool HALF>
+__global__ __launch_bounds__(kPagedThreads) void paged_few_kernel(PagedAttnArgs a) {
+    using F = Few<DP>;
+    __shared__ float joint[kPagedWaves][16][F::Row];
+    const int lane = lane_id(), c = lane & 15, g = lane >> 4, wave = int(threadIdx.x) >> 6;
+    const int split = int(blockIdx.x), head = int(blockIdx.y) % a.n_kv, tile = int(blockIdx.y) / a.n_kv,
+              seq = int(blockIdx.z);
+    Rows r;
+    find_rows(a, seq, split, tile, 16, r);
+    const int r0 = 16 * tile;
+    if (r0 >= r.count || !r.used) return;
+    const int row = r0 + c, limit = row_limit(a, r, row);
+    const int low = row_limit(a, r, r0); // the tile's fewest tokens
+    const int32_t *table = a.batch.table + (a.shared ? 0 : int64_t(seq) * a.batch.table_stride);
+    const uint16_t *kh = a.pool.k + int64_t(head) * a.pool.k_head;
+    const uint16_t *vh = a.pool.v + int64_t(head) * a.pool.v_head;
+    const int vc = min(F::C * c, a.dim - F::C);
+    // the row's queries: channels 32 i + 8 g ..
+    u32x4a q[F::KS];
+    {
+        const uint16_t *qr = a.q.p + int64_t(row_token(a, r, min(row, r.count - 1))) * a.q.token +
+                             int64_t(head * a.group + min(row, r.count - 1) % a.group) * a.q.head;
+#pragma unroll
+        for (int i = 0; i < F::KS; ++i) {
+            const int ch = 32 * i + 8 * g;
+            q[i] = row < r.count && ch < a.dim ? *reinterpret_cast<const u32x4a *>(qr + ch) : u32x4a{0, 0, 0, 0};
+        }
+    }
+    f32x4 acc[F::C];
+#pragma unroll
+    for (int j = 0; j < F::C; ++j) acc[j] = f32x4{0, 0, 0, 0};
+    float m = -__builtin_inff(), l = 0.0f;
+    for (int tok = r.t0 + 32 * wave; tok < r.t1; tok += 32 * kPagedWaves) {
+        FewTile<DP> f;
+        few_load<DP>(a, r, table, kh, vh, tok, vc, f);
+        f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+        for (int i = 0; i < F::KS; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) s[j] = mfma16<HALF>(f.k[j][i], q[i], s[j]);
+        float p[8];
+        const bool cut = tok + 32 > low || tok + 32 > r.t1; // some row does not see some of these tokens
+#pragma unroll
+        for (int n = 0; n < 8; ++n) p[n] = s[n >> 2][n & 3] * a.scale2;
+        const int seen = min(limit, r.t1) - (tok + 4 * g); // lane's token n is seen if off(n) < seen
+        if (cut) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                if ((n & 3) + 16 * (n >> 2) >= seen) p[n] = -__builtin_inff();
+        }
+        float t = p[0];
+#pragma unroll
+        for (int n = 1; n < 8; ++n) t = fmaxf(t, p[n]);
+        t = fmaxf(t, __shfl_xor(t, 16));
+        t = fmaxf(t, __shfl_xor(t, 32));
+        const float mn = fmaxf(m, t);
+        const float base = mn == -__builtin_inff() ? 0.0f : mn;
+        const float alpha = exp2_f32(m - base);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            p[n] = exp2_f32(p[n] - base);
+            l += p[n];
+        }
+#pragma unroll
+        for (int j = 0; j < F::C; ++j) acc[j] *= alpha;
+        // P as the sum of two 16-bit numbers (16 bits of it, so that an
+        // output's error stays its own rounding; the pass waits for memory)
+        u32x4a hi, lo;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            hi[n] = pack2<HALF>(p[2 * n], p[2 * n + 1]);
+            lo[n] = pack2<HALF>(p[2 * n] - low_f32<HALF>(hi[n]), p[2 * n + 1] - high_f32<HALF>(hi[n]));
+        }
+        bool wild = false;
+        if (cut) {
+            bool w = false;
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+#pragma unroll
+                for (int k = 0; k < F::VW; ++k) w |= wild2<HALF>(f.v[n][k]);
+            wild = __ballot(w) != 0;
+        }
+        if (!wild) {
+#pragma unroll
+            for (int j = 0; j < F::C; ++j) {
+                const u32x4a v = few_v<DP>(f, j);
+                acc[j] = mfma16<HALF>(v, hi, acc[j]);
+                acc[j] = mfma16<HALF>(v, lo, acc[j]);
+            }
+        } else {
+            // An infinity or NaN among these tokens' V, and rows that do not
+            // see all of them: a token at a time, so that 0 times it stays out
+            // of the rows that do not see it.
+            for (int u = 0; u < 32; ++u) {
+                const int ug = (u >> 2) & 3, un = (u & 3) + 4 * (u >> 4); // its lane group and place there
+                const bool see = tok + u < limit && tok + u < r.t1;
+                const uint32_t keep = g == ug ? (un & 1 ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
+                u32x4a h = u32x4a{0, 0, 0, 0}, w = u32x4a{0, 0, 0, 0};
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const uint32_t k = n == (un >> 1) ? keep : 0u;
+                    h[n] = hi[n] & k;
+                    w[n] = lo[n] & k;
+                }
+#pragma unroll
+                for (int j = 0; j < F::C; ++j) {
+                    u32x4a v = few_v<DP>(f, j);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) v[n] &= n == (un >> 1) ? keep : 0u;
+                    f32x4 x = mfma16<HALF>(v, h, acc[j]);
+                    x = mfma16<HALF>(v, w, x);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[j][k] = see ? x[k] : acc[j][k];
+                }
+            }
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    // the waves' states to LDS: lane (c, g) holds row c, channels
+    // min(C (4 g + i), dim - C) + j
+    const int rows = min(16, r.count - r0);
+    if (g == 0) {
+        joint[wave][c][F::JC] = m;
+        joint[wave][c][F::JC + 1] = l;
+    }
+    for (int d0 = 0; d0 < a.dim; d0 += F::JC) {
+        if (d0 > 0) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int ch = min(F::C * (4 * g + i), a.dim - F::C) - d0;
+#pragma unroll
+            for (int j = 0; j < F::C; ++j)
+                if (F::JC == DP || uint32_t(ch + j) < uint32_t(F::JC)) joint[wave][c][ch + j] = acc[j][i];
+        }
+        __syncthreads();
+        const int nd = min(F::JC, a.dim - d0);
+        for (int i = int(threadIdx.x); i < rows * nd; i += kPagedThreads) {
+            const int rr = i / nd, d = i - rr * nd;
+            float M = -__builtin_inff();
+#pragma unroll
+            for (int w = 0; w < kPagedWaves; ++w) M = fmaxf(M, joint[w][rr][F::JC]);
+            const float base = M == -__builtin_inff() ? 0.0f : M;
+            float L = 0.0f, A = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kPagedWaves; ++w) {
+                const float e = exp2_f32(joint[w][rr][F::JC] - base);
+                // a wave without tokens for the row (l 0) adds nothing
+                const float lw = joint[w][rr][F::JC + 1];
+                L += lw == 0.0f ? 0.0f : lw * e;
+                A += lw == 0.0f ? 0.0f : joint[w][rr][d] * e;
+            }
+            write_state<HALF>(a, r, head, split, r0 + rr, d0 + d, M, L, A);
+        }
+    }
+}
+
+// -------------------------------------------------------------- many rows --
+// Up to 128 query rows per workgroup, 32 per wave (32 x 32 x 16 products):
+// prompts in chunks, draft tokens, and the rows of a whole batch against a
+// shared prefix. A tile of tokens (64 up to head_dim 128, 32 above) is staged
+// in LDS, once for all rows: pages as they are, containers decoded on the way
+// (SRC 1). Rows of K are read from LDS as they lie; V's operand, four tokens of
+// one channel per lane, by the transposing read. P is rounded once to 16 bits:
+// the second product would else cost twice, and the error that this leaves in
+// an output (a sum of independent roundings) is as large as the output's own
+// rounding.
+template <int DP>
+struct Many {
+    static constexpr int KT = tile_tokens(DP);
+    static constexpr int ST = KT / 32;                        // score tiles
+    static constexpr int KS = DP / 16;                        // steps of 16 channels
+    static constexpr int CT = DP / 32;                        // channel tiles of the output
+    static constexpr int KR = DP + 8;                         // LDS elements per row of K: rows 4 banks apart
+    static constexpr int VR = DP + (DP % 64 == 0 ? 32 : 0);   // of V: four rows 16 banks apart
+    static constexpr int PR = DP / 8;                         // 16-byte pieces per row
+    static constexpr int Occ = DP <= 96 ? 2 : 1;              // waves per SIMD that the registers allow
+    static constexpr int NP = KT * PR / kPagedThreads;        // pieces per thread
+    static_assert(KT * PR % kPagedThreads == 0, "whole pieces per thread");
+};
+
+template <int DP>
+struct alignas(16) ManyLds {
+    uint16_t k[Many<DP>::KT * Many<DP>::KR];
+    uint16_t v[Many<DP>::KT * Many<DP>::VR];
+    int2 row[Many<DP>::KT]; // page and place of the next tile's tokens
+};
+
+typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t any_u32x2 __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t any_u32 __attribute__((aligned(1)));
+typedef uint16_t any_u16 __attribute__((aligned(1)));
+
+// Two elements of a coded row: bytes b and b + 1 of sm and of base, with their codes.
+__device__ __forceinline__ uint32_t join_pair(uint32_t sm, uint32_t base, int b, uint32_t c0, uint32_t c1) {
+    return bf16_join(((base >> (8 * b)) & 0xFFu) + c0, (sm >> (8 * b)) & 0xFFu) |
+           (bf16_join(((base >> (8 * b + 8)) & 0xFFu) + c1, (sm >> (8 * b + 8)) & 0xFFu) << 16);
+}
+
+// Eight channels from channel `ch` of row `row` of a segment (escapes come after).
+__device__ __forceinline__ u32x4a seg_octet(const PrefixSeg &s, int dim, int row, int ch) {
+    const int e = (s.row0 + row) * dim + ch; // element of the block
+    if (s.mode == 0) {
+        const any_u32x4 v = *reinterpret_cast<const any_u32x4 *>(s.data + 2 * e);
+        return u32x4a{v.x, v.y, v.z, v.w};
+    }
+    const any_u32x2 base = *reinterpret_cast<const any_u32x2 *>(s.data + ch);
+    const any_u32x2 sm = *reinterpret_cast<const any_u32x2 *>(s.data + dim + e);
+    const uint8_t *cp = s.data + dim + s.n_tokens * dim + (e >> 3) * s.mode;
+    uint32_t c;
+    if (s.mode == 4) c = *reinterpret_cast<const any_u32 *>(cp);
+    else if (s.mode == 2) c = *reinterpret_cast<const any_u16 *>(cp);
+    else c = uint32_t(cp[0]) | (uint32_t(cp[1]) << 8) | (uint32_t(cp[2]) << 16);
+    const uint32_t mask = (1u << s.mode) - 1u;
+    auto code = [&](int i) { return (c >> (s.mode * i)) & mask; };
+    return u32x4a{join_pair(sm.x, base.x, 0, code(0), code(1)), join_pair(sm.x, base.x, 2, code(2), code(3)),
+                  join_pair(sm.y, base.y, 0, code(4), code(5)), join_pair(sm.y, base.y, 2, code(6), code(7))};
+}
+
+// A tile of a container tensor to LDS rows of R elements; V: rows past the
+// tile's tokens are zero.
+template <int R, int KT, bool V>
+__device__ __forceinline__ void stage_coded(const PrefixTensor &t, int tile, int dim, int rows, uint16_t *lds) {
+    const int pr = dim / 8;
+    for (int s = t.tile_seg[tile]; s < t.tile_seg[tile + 1]; ++s) {
+        const PrefixSeg seg = t.segs[s];
+        for (int o = int(threadIdx.x); o < seg.rows * pr; o += kPagedThreads) {
+            const int row = o / pr, ch = 8 * (o - row * pr);
+            *reinterpret_cast<u32x4a *>(lds + (seg.dst + row) * R + ch) = seg_octet(seg, dim, row, ch);
+        }
+    }
+    if (V)
+        for (int o = rows * pr + int(threadIdx.x); o < KT * pr; o += kPagedThreads) {
+            const int row = o / pr, ch = 8 * (o - row * pr);
+            *reinterpret_cast<u32x4a *>(lds + row * R + ch) = u32x4a{0, 0, 0, 0};
+        }
+}
+// The tile's escapes over their elements.
+template <int R>
+__device__ __forceinline__ void patch_coded(const PrefixTensor &t, int tile, int dim, uint16_t *lds) {
+    for (int s = t.tile_seg[tile]; s < t.tile_seg[tile + 1]; ++s) {
+        const PrefixSeg seg = t.segs[s];
+        for (int i = int(threadIdx.x); i < seg.n_esc; i += kPagedThreads) {
+            const uint32_t rec = seg.esc[i];
+            const int e = int(rec & 0xFFFFu), row = e / dim - seg.row0;
+            if (uint32_t(row) < uint32_t(seg.rows)) // (a damaged container's records)
+                lds[(seg.dst + row) * R + (e - (row + seg.row0) * dim)] = uint16_t(rec >> 16);
+        }
+    }
+}
+
+template <int DP, bool HALF, int SRC>
+__global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(Many<DP>::Occ, Many<DP>::Occ))) void
+paged_many_kernel(PagedAttnArgs a) {
+    using S = Many<DP>;
+    __shared__ ManyLds<DP> lds;
+    const int tid = int(threadIdx.x), lane = lane_id(), wave = tid >> 6, c = lane & 31, h = lane >> 5;
+    const int split = int(blockIdx.x), head = int(blockIdx.y) % a.n_kv, tile = int(blockIdx.y) / a.n_kv,
+              seq = int(blockIdx.z);
+    Rows r;
+    find_rows(a, seq, split, tile, 32 * kPagedWaves, r);
+    if (32 * kPagedWaves * tile >= r.count || !r.used) return;
+    const int r0 = 32 * (kPagedWaves * tile + wave);
+    const int row = r0 + c, limit = row_limit(a, r, row);
+    const bool busy = r0 < r.count;
+    const int low = row_limit(a, r, min(r0, r.count - 1)); // the wave's fewest tokens
+    const int wg_low = row_limit(a, r, 32 * kPagedWaves * tile);
+    const int32_t *table = a.batch.table + (a.shared ? 0 : int64_t(seq) * a.batch.table_stride);
+    const uint16_t *kh = a.pool.k + int64_t(head) * a.pool.k_head;
+    const uint16_t *vh = a.pool.v + int64_t(head) * a.pool.v_head;
+    // channels past head_dim: K's are zero (they meet zero queries), V's feed outputs that nobody reads
+    for (int i = tid; i < S::KT * (DP - a.dim); i += kPagedThreads) {
+        const int t = i / (DP - a.dim), d = a.dim + i - t * (DP - a.dim);
+        lds.k[t * S::KR + d] = 0;
+        lds.v[t * S::VR + d] = 0;
+    }
+    u32x4a q[S::KS];
+    {
+        const int rr = min(row, r.count - 1);
+        const uint16_t *qr = a.q.p + int64_t(row_token(a, r, rr)) * a.q.token +
+                             int64_t(head * a.group + rr % a.group) * a.q.head;
+#pragma unroll
+        for (int i = 0; i < S::KS; ++i) {
+            const int ch = 16 * i + 8 * h;
+            q[i] = row < r.count && ch < a.dim ? *reinterpret_cast<const u32x4a *>(qr + ch) : u32x4a{0, 0, 0, 0};
+        }
+    }
+    f32x16 acc[S::CT];
+#pragma unroll
+    for (int j = 0; j < S::CT; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[j][i] = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f;
+
+    // the next tile's rows on their way (pages)
+    u32x4a kn[S::NP], vn[S::NP];
+    auto find = [&](int tok) { // page and place of token tok + tid
+        int2 p = make_int2(0, 0);
+        if (tid < S::KT && tok < r.t1) p.x = page_at(a, table, min(tok + tid, r.t1 - 1), p.y);
+        return p;
+    };
+    auto request = [&](int tok) {
+#pragma unroll
+        for (int k = 0; k < S::NP; ++k) {
+            const int o = tid + kPagedThreads * k, t = o / S::PR, ch = 8 * (o - t * S::PR);
+            const int2 at = lds.row[t];
+            kn[k] = vn[k] = u32x4a{0, 0, 0, 0};
+            if (ch < a.dim) {
+                kn[k] = *reinterpret_cast<const u32x4a *>(kh + int64_t(at.x) * a.pool.k_page +
+                                                          int64_t(at.y) * a.pool.k_token + ch);
+                if (tok + t < r.t1)
+                    vn[k] = *reinterpret_cast<const u32x4a *>(vh + int64_t(at.x) * a.pool.v_page +
+                                                              int64_t(at.y) * a.pool.v_token + ch);
+            }
+        }
+    };
+    if constexpr (SRC == 0) {
+        if (r.t0 < r.t1) {
+            const int2 p = find(r.t0);
+            if (tid < S::KT) lds.row[tid] = p;
+            __syncthreads();
+            request(r.t0);
+        }
+    }
+    for (int tok = r.t0; tok < r.t1; tok += S::KT) {
+        int2 next = make_int2(0, 0);
+        if constexpr (SRC == 0) next = find(tok + S::KT);
+        __syncthreads(); // the last tile is read
+        bool w = false;
+        const bool wg_cut = tok + S::KT > wg_low;
+        if constexpr (SRC == 0) {
+#pragma unroll
+            for (int k = 0; k < S::NP; ++k) {
+                const int o = tid + kPagedThreads * k, t = o / S::PR, ch = 8 * (o - t * S::PR);
+                if (ch < a.dim) {
+                    *reinterpret_cast<u32x4a *>(lds.k + t * S::KR + ch) = kn[k];
+                    *reinterpret_cast<u32x4a *>(lds.v + t * S::VR + ch) = vn[k];
+                }
+                if (wg_cut)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w |= wild2<HALF>(vn[k][i]);
+            }
+            if (tid < S::KT) lds.row[tid] = next;
+        } else {
+            const PrefixTensor pk = a.px[2 * head], pv = a.px[2 * head + 1];
+            const int pt = tok / S::KT, rows = min(S::KT, r.len - tok);
+            stage_coded<S::KR, S::KT, false>(pk, pt, a.dim, rows, lds.k);
+            stage_coded<S::VR, S::KT, true>(pv, pt, a.dim, rows, lds.v);
+            __syncthreads();
+            patch_coded<S::KR>(pk, pt, a.dim, lds.k);
+            patch_coded<S::VR>(pv, pt, a.dim, lds.v);
+        }
+        bool wild = false;
+        if (SRC == 0 && wg_cut) wild = __syncthreads_or(w) != 0;
+        else __syncthreads();
+        if constexpr (SRC == 0)
+            if (tok + S::KT < r.t1) request(tok + S::KT);
+        if (!busy) continue;
+        f32x16 s[S::ST];
+#pragma unroll
+        for (int t = 0; t < S::ST; ++t) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < S::KS; ++i) {
+                const u32x4a kf = *reinterpret_cast<const u32x4a *>(lds.k + (32 * t + c) * S::KR + 16 * i + 8 * h);
+                s[t] = mfma32<HALF>(kf, q[i], s[t]);
+            }
+        }
+        // element i of tile t: token tok + 32 t + 8 (i / 4) + 4 h + i % 4
+        const int seen = min(limit, r.t1) - tok - 4 * h;
+        const bool cut = tok + S::KT > min(low, r.t1);
+        float mt = -__builtin_inff();
+#pragma unroll
+        for (int t = 0; t < S::ST; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[t][i] *= a.scale2;
+                if (cut && 32 * t + 8 * (i >> 2) + (i & 3) >= seen) s[t][i] = -__builtin_inff();
+                mt = fmaxf(mt, s[t][i]);
+            }
+        mt = fmaxf(mt, __shfl_xor(mt, 32));
+        const float mn = fmaxf(m, mt);
+        const float base = mn == -__builtin_inff() ? 0.0f : mn;
+        const float alpha = exp2_f32(m - base);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < S::ST; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[t][i] = exp2_f32(s[t][i] - base);
+                l += s[t][i];
+            }
+#pragma unroll
+        for (int j = 0; j < S::CT; ++j) acc[j] *= alpha;
+        // V: lane group lane / 16 reads channels 16 (group % 2) .. of tokens 4 (group / 2) ..
+        const uint16_t *vb = lds.v + ((lane & 15) >> 2) * S::VR + 4 * h * S::VR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        if (wild) {
+            // An infinity or NaN among these tokens' V, and rows that do not
+            // see all of them: a token at a time on the vector ALU, added only
+            // where the row sees it, so that 0 times it stays out of the others.
+#pragma unroll 1
+            for (int u = 0; u < S::KT; ++u) {
+                float pu = 0.0f;
+#pragma unroll
+                for (int t = 0; t < S::ST; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) pu = 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) == u ? s[t][i] : pu;
+                pu += __shfl_xor(pu, 32); // (the other half of the lanes does not hold it)
+                if (tok + u >= limit || tok + u >= r.t1) continue;
+                const uint16_t *vu = lds.v + u * S::VR + 4 * h;
+#pragma unroll
+                for (int j = 0; j < S::CT; ++j)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        acc[j][i] = __builtin_fmaf(pu, low_f32<HALF>(vu[32 * j + 8 * (i >> 2) + (i & 3)]), acc[j][i]);
+            }
+            continue;
+        }
+#pragma unroll
+        for (int t = 0; t < S::ST; ++t)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) { // 16 tokens
+                u32x4a p;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) p[n] = pack2<HALF>(s[t][8 * k + 2 * n], s[t][8 * k + 2 * n + 1]);
+#pragma unroll
+                for (int j = 0; j < S::CT; ++j) {
+                    const uint16_t *at = vb + (32 * t + 16 * k) * S::VR + 32 * j;
+                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at));
+                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 8 * S::VR));
+                    const uint2 x = __builtin_bit_cast(uint2, v0), y = __builtin_bit_cast(uint2, v1);
+                    acc[j] = mfma32<HALF>(u32x4a{x.x, x.y, y.x, y.y}, p, acc[j]);
+                }
+            }
+    }
+    if (!busy) return;
+    l += __shfl_xor(l, 32);
+    if (row >= r.count) return;
+    // lane (c, h): row c, channels 32 j + 8 i + 4 h .. + 3
+    const int64_t slot = state_slot(a, r, head, split, row);
+    const int64_t tok = row_token(a, r, row);
+    const int hq = head * a.group + row % a.group;
+    if (h == 0) {
+        if (a.direct) {
+            if (a.lse != nullptr) a.lse[tok * (a.n_kv * a.group) + hq] = log_sum(m, l);
+        } else {
+            a.ml[2 * slot] = m;
+            a.ml[2 * slot + 1] = l;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < S::CT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int ch = 32 * j + 8 * i + 4 * h;
+            if (ch >= a.dim) continue;
+            if (a.direct) {
+                uint2 w;
+                w.x = pack2<HALF>(finish(acc[j][4 * i], l), finish(acc[j][4 * i + 1], l));
+                w.y = pack2<HALF>(finish(acc[j][4 * i + 2], l), finish(acc[j][4 * i + 3], l));
+                *reinterpret_cast<uint2 *>(a.out.p + tok * a.out.token + int64_t(hq) * a.out.head + ch) = w;
+            } else {
+                *reinterpret_cast<float4 *>(a.acc + slot * a.dim + ch) =
+                    make_float4(acc[j][4 * i], acc[j][4 * i + 1], acc[j][4 * i + 2], acc[j][4 * i + 3]);
+            }
+        }
+}
+
+} // namespace paged
+} // namespace kvexp_dev

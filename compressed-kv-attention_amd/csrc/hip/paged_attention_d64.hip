@@ -1,0 +1,6 @@
+// Attention over a paged cache, channels held as 64 (paged_attention.h).
+#include "paged_attention_launch.h"
+
+namespace kvexp_launch {
+KVEXP_PAGED_LAUNCH(64)
+} // namespace kvexp_launch

@@ -1,0 +1,167 @@
+// Joins the partial states of the paged attention kernels, and picks their
+// instantiation.
+#include "paged_attention.h"
+
+#include <algorithm>
+
+namespace kvexp_dev {
+namespace paged {
+namespace {
+
+// Joins the states of a row: maximum, then the weighted sums. One wave per
+// row; lane s takes the weight of split s of a batch of 64, then every lane
+// its channels of the batch's rows, in split order (the same sum every time).
+struct Joined {
+    float m = -__builtin_inff(), l = 0.0f;
+    float acc[4] = {0, 0, 0, 0};
+};
+
+__device__ __forceinline__ float wave_max_all(float x) {
+    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+    return x;
+}
+__device__ __forceinline__ float wave_sum_all(float x) {
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+    return x;
+}
+
+__device__ __forceinline__ void join(Joined &j, const float *acc, const float *ml, int64_t slot, int64_t step, int n,
+                                     int dim) {
+    const int lane = lane_id();
+    for (int s0 = 0; s0 < n; s0 += kWave) {
+        const int cnt = min(kWave, n - s0);
+        float m = -__builtin_inff(), l = 0.0f;
+        if (lane < cnt) {
+            const float2 x = *reinterpret_cast<const float2 *>(ml + 2 * (slot + (s0 + lane) * step));
+            m = x.x;
+            l = x.y;
+        }
+        const float mn = fmaxf(j.m, wave_max_all(l == 0.0f ? -__builtin_inff() : m));
+        const float base = mn == -__builtin_inff() ? 0.0f : mn;
+        const float old = exp2_f32(j.m - base), w = l == 0.0f ? 0.0f : exp2_f32(m - base);
+        j.m = mn;
+        j.l = j.l * old + wave_sum_all(l == 0.0f ? 0.0f : w * l);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) j.acc[k] *= old;
+#pragma unroll 4
+        for (int i = 0; i < cnt; ++i) {
+            const float wi = readlane_f32(w, i), li = readlane_f32(l, i);
+            if (li == 0.0f) continue; // nothing there (its sums were not written)
+            const float *row = acc + (slot + (s0 + i) * step) * dim;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int d = lane + kWave * k;
+                if (d < dim) j.acc[k] = __builtin_fmaf(wi, row[d], j.acc[k]);
+            }
+        }
+    }
+}
+
+// Fills in a shared prefix's segments (the host left each one's tensor in
+// n_esc and its block in mode): the block's payload and header fields, and the
+// records of the segment's rows (a block's records ascend by element).
+__global__ __launch_bounds__(256) void prefix_segs_kernel(PrefixSeg *__restrict__ segs, int n,
+                                                          const EscJob *__restrict__ jobs) {
+    const int i = int(blockIdx.x) * 256 + int(threadIdx.x);
+    if (i >= n) return;
+    PrefixSeg s = segs[i];
+    const EscJob j = jobs[s.n_esc];
+    const int b = s.mode;
+    const uint8_t *p = j.blob + j.offs[b];
+    const BlockHdr h = read_hdr(p);
+    const uint32_t *rec = j.pos + j.esc0[b];
+    const int n_rec = j.esc0[b + 1] - j.esc0[b];
+    auto below = [&](int e) { // records of elements below e
+        int lo = 0, hi = n_rec;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (int(rec[mid] & 0xFFFFu) < e) lo = mid + 1;
+            else hi = mid;
+        }
+        return lo;
+    };
+    const int r0 = below(s.row0 * j.dim), r1 = below((s.row0 + s.rows) * j.dim);
+    s.data = p + 8;
+    s.esc = rec + r0;
+    s.n_esc = max(r1 - r0, 0);
+    s.mode = h.mode;
+    s.n_tokens = h.n_tokens;
+    segs[i] = s;
+}
+
+template <bool HALF>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a, int rows_per_seq) {
+    const int hq_all = a.n_kv * a.group;
+    const int64_t w = int64_t(blockIdx.x) * 4 + (int(threadIdx.x) >> 6);
+    const int seq = int(w / rows_per_seq);
+    if (seq >= a.batch.n_seqs) return;
+    const int rest = int(w - int64_t(seq) * rows_per_seq);
+    const int i = rest / hq_all, hq = rest - i * hq_all;
+    Rows r;
+    find_rows(a, seq, 1, 1, 1, r); // (split and tile 1: no errors raised here)
+    if (i >= r.n) return;
+    const int head = hq / a.group, g = hq - head * a.group;
+    const int row = i * a.group + g;
+    const int64_t tok = r.first + i;
+    Joined j;
+    if (a.s_splits > 0) {
+        const int len = split_tokens(a.s_len, a.s_splits, a.s_min_split);
+        const int n = max(1, (a.s_len + len - 1) / len);
+        join(j, a.s_acc, a.s_ml, int64_t(head) * a.s_splits * a.s_rows + tok * a.group + g, a.s_rows, n, a.dim);
+    }
+    const int n = max(1, (r.len + r.split_len - 1) / r.split_len);
+    join(j, a.acc, a.ml, state_slot(a, r, head, 0, row), a.max_rows, n, a.dim);
+    const int lane = lane_id();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int d = lane + kWave * k;
+        if (d < a.dim) a.out.p[tok * a.out.token + int64_t(hq) * a.out.head + d] = to_16<HALF>(finish(j.acc[k], j.l));
+    }
+    if (lane == 0 && a.lse != nullptr) a.lse[tok * hq_all + hq] = log_sum(j.m, j.l);
+}
+
+} // namespace
+} // namespace paged
+} // namespace kvexp_dev
+
+namespace kvexp_launch {
+
+using namespace kvexp_dev;
+
+#define KVEXP_PAGED_DECL(DP)                                                                       \
+    hipError_t paged_few_d##DP(const PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s);      \
+    hipError_t paged_many_d##DP(const PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s);
+KVEXP_PAGED_DECL(32)
+KVEXP_PAGED_DECL(64)
+KVEXP_PAGED_DECL(96)
+KVEXP_PAGED_DECL(128)
+KVEXP_PAGED_DECL(192)
+KVEXP_PAGED_DECL(256)
+
+hipError_t paged_attention(const PagedAttnArgs &a, bool half, bool many, int n_seqs, hipStream_t s) {
+#define KVEXP_PAGED_PICK(DP) \
+    if (a.dim <= DP) return many ? paged_many_d##DP(a, half, n_seqs, s) : paged_few_d##DP(a, half, n_seqs, s);
+    KVEXP_PAGED_PICK(32)
+    KVEXP_PAGED_PICK(64)
+    KVEXP_PAGED_PICK(96)
+    KVEXP_PAGED_PICK(128)
+    KVEXP_PAGED_PICK(192)
+    KVEXP_PAGED_PICK(256)
+    return hipErrorInvalidValue;
+}
+
+hipError_t prefix_segs(PrefixSeg *segs, int n, const EscJob *jobs, hipStream_t s) {
+    hipLaunchKernelGGL(paged::prefix_segs_kernel, dim3(unsigned((n + 255) / 256)), dim3(256), 0, s, segs, n, jobs);
+    return hipGetLastError();
+}
+
+hipError_t paged_merge(const PagedAttnArgs &a, bool half, hipStream_t s) {
+    const int rows = a.batch.max_new * a.n_kv * a.group;
+    const int64_t waves = int64_t(a.batch.n_seqs) * rows;
+    const dim3 grid(unsigned((waves + 3) / 4));
+    if (half) hipLaunchKernelGGL(paged::paged_merge_kernel<true>, grid, dim3(256), 0, s, a, rows);
+    else hipLaunchKernelGGL(paged::paged_merge_kernel<false>, grid, dim3(256), 0, s, a, rows);
+    return hipGetLastError();
+}
+
+} // namespace kvexp_launch

@@ -15,6 +15,9 @@ import os
 import re
 from dataclasses import dataclass
 
+from . import paged as _paged
+from .paged import Batch, PagedCache, PagePrefix, Prefix, Rope  # noqa: F401
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
@@ -117,6 +120,7 @@ def lib() -> C.CDLL:
     L.kvexp_hip_plan_kernel_time.argtypes = [vp, C.POINTER(C.c_double), C.POINTER(C.c_int)]
     L.kvexp_hip_attention_decode_host.argtypes = [vp, i32, vp, vp, vp, vp, sz, vp, sz, vp, i32, i32, i32, i32, i32]
     L.kvexp_hip_expf.argtypes = [vp, vp, vp, sz, vp]
+    _paged.declare(L, _Head)
     _lib = L
     return L
 
@@ -360,6 +364,19 @@ class Context:
                                      enc.n_blocks, seq, enc.dim, _ptr(out), 1 if check_errors else 0,
                                      _stream(stream)))
         return out[: seq * enc.dim]
+
+    # paged cache --------------------------------------------------------------
+    def rope(self, x, positions, rope: Rope, out=None, inverse: bool = False, stream=None):
+        """x [tokens, heads, head_dim] rotated (paged.rope)."""
+        return _paged.rope(self, x, positions, rope, out, inverse, stream)
+
+    def paged_cache(self, n_heads: int, dim: int, n_pages: int, page_tokens: int = 64, dtype=None) -> PagedCache:
+        """An empty cache of n_pages pages of page_tokens tokens."""
+        return PagedCache(self, n_heads, dim, n_pages, page_tokens, dtype)
+
+    def prefix(self, ks: list, vs: list, stream=None) -> Prefix:
+        """Containers (one K and one V per KV head) as a prefix that batches of a paged cache share."""
+        return Prefix(self, ks, vs, stream)
 
     # attention --------------------------------------------------------------
     def plan(self, heads: list, n_q: int, dim: int, split: int = 128, order: int = ORDER_SCALAR,

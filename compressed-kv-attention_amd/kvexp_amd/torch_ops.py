@@ -32,7 +32,7 @@ from collections import OrderedDict
 import torch
 from torch import Tensor
 
-from . import ORDER_SCALAR, Context, Encoded
+from . import ORDER_SCALAR, Batch, Context, Encoded, PagedCache, Prefix, Rope
 
 _contexts: dict[int, Context] = {}
 _plans: "OrderedDict[tuple, object]" = OrderedDict()
@@ -258,3 +258,123 @@ def decode_attention_containers(q: Tensor, ks: list, vs: list, seqs: list[int], 
         q, [e.blob for e in ks], [e.offsets for e in ks], [e.first for e in ks], [e.blob for e in vs],
         [e.offsets for e in vs], [e.first for e in vs], [int(e.nbytes) for e in ks], [int(e.nbytes) for e in vs],
         [int(s) for s in seqs], int(n_splits), int(split_tokens), int(order), bool(reuse_plan))
+
+
+# ---- rotary positions and the paged cache --------------------------------
+# The operators take the pools and index tensors themselves (a cache's k, v and
+# status word), so that they trace; kvexp_amd.PagedCache makes the same calls.
+def _rope_of(inv_freq: Tensor, axes: Tensor | None, interleaved: bool, scale: float) -> Rope:
+    return Rope(inv_freq, axes, interleaved, scale)
+
+
+@torch.library.custom_op("kvexp::rope", mutates_args=())
+def rope(x: Tensor, positions: Tensor | None, inv_freq: Tensor, axes: Tensor | None = None, interleaved: bool = False,
+         scale: float = 1.0, inverse: bool = False) -> Tensor:
+    """x [tokens, heads, head_dim] with its first 2 n channels rotated (Context.rope); differentiable in x."""
+    if x.device.type != "cuda":
+        raise ValueError("kvexp.rope: x must be a ROCm device tensor")
+    return _context(x.device).rope(x, positions, _rope_of(inv_freq, axes, interleaved, scale), inverse=inverse)
+
+
+@rope.register_fake
+def _(x, positions, inv_freq, axes=None, interleaved=False, scale=1.0, inverse=False):
+    return x.new_empty(x.shape)
+
+
+def _rope_setup(ctx, inputs, output):
+    _, positions, inv_freq, axes, ctx.interleaved, ctx.scale, ctx.inverse = inputs
+    ctx.save_for_backward(*(t for t in (positions, inv_freq, axes) if t is not None))
+    ctx.held = (positions is not None, axes is not None)
+
+
+def _rope_backward(ctx, dy):
+    # the rotation's transpose is the rotation back, with the same scale
+    saved = list(ctx.saved_tensors)
+    positions = saved.pop(0) if ctx.held[0] else None
+    inv_freq = saved.pop(0)
+    axes = saved.pop(0) if ctx.held[1] else None
+    dx = torch.ops.kvexp.rope(dy, positions, inv_freq, axes, ctx.interleaved, ctx.scale, not ctx.inverse)
+    return dx, None, None, None, None, None, None
+
+
+rope.register_autograd(_rope_backward, setup_context=_rope_setup)
+
+
+def _paged(k_pages: Tensor, v_pages: Tensor, status: Tensor) -> PagedCache:
+    if k_pages.device.type != "cuda":
+        raise ValueError("kvexp.paged: the pages must be ROCm device tensors")
+    if k_pages.dim() != 4:
+        raise ValueError("kvexp.paged: pages must be [n_pages, n_heads, page_tokens, head_dim]")
+    if status.dtype != torch.int32 or status.numel() != 1 or status.device != k_pages.device:
+        raise ValueError("kvexp.paged: status must be an int32 word on the pages' device")
+    p, h, t, d = k_pages.shape
+    cache = PagedCache(_context(k_pages.device), h, d, p, t, k_pages.dtype, k=k_pages, v=v_pages)
+    cache.status_word = status
+    return cache
+
+
+@torch.library.custom_op("kvexp::paged_append", mutates_args=("k_pages", "v_pages", "status"))
+def paged_append(k_pages: Tensor, v_pages: Tensor, status: Tensor, k: Tensor, v: Tensor, table: Tensor, lens: Tensor,
+                 starts: Tensor | None, q: Tensor, inv_freq: Tensor, axes: Tensor | None = None,
+                 positions: Tensor | None = None, offset: int = 0, interleaved: bool = False,
+                 scale: float = 1.0) -> Tensor:
+    """PagedCache.append: new keys (rotated) and values to their pages; returns the queries rotated."""
+    cache = _paged(k_pages, v_pages, status)
+    return cache.append(k, v, Batch(table, lens, starts), _rope_of(inv_freq, axes, interleaved, scale), positions,
+                        offset, q=q)
+
+
+@paged_append.register_fake
+def _(k_pages, v_pages, status, k, v, table, lens, starts, q, inv_freq, axes=None, positions=None, offset=0,
+      interleaved=False, scale=1.0):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("kvexp::paged_attention", mutates_args=("status",))
+def paged_attention(k_pages: Tensor, v_pages: Tensor, status: Tensor, q: Tensor, table: Tensor, lens: Tensor,
+                    starts: Tensor | None, scale: float, max_new: int = 0, max_len: int = 0,
+                    prefix_table: Tensor | None = None, prefix_len: int = 0) -> tuple[Tensor, Tensor]:
+    """PagedCache.attention, with a shared prefix in pages where prefix_table is given: (out, lse)."""
+    cache = _paged(k_pages, v_pages, status)
+    prefix = None if prefix_table is None else cache.prefix(prefix_table, prefix_len)
+    return cache.attention(q, Batch(table, lens, starts, max_new, max_len), scale, prefix, return_lse=True)
+
+
+@paged_attention.register_fake
+def _(k_pages, v_pages, status, q, table, lens, starts, scale, max_new=0, max_len=0, prefix_table=None, prefix_len=0):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+_prefixes: dict[int, Prefix] = {}
+
+
+def register_prefix(ks: list, vs: list) -> int:
+    """Registers containers (one K and one V per KV head, on one device) as a shared prefix for
+    torch.ops.kvexp.prefix_attention; returns the handle. They must not change while registered."""
+    h = 1 + max(_prefixes, default=0)
+    _prefixes[h] = _context(ks[0].blob.device).prefix(ks, vs)
+    return h
+
+
+def unregister_prefix(handle: int) -> None:
+    p = _prefixes.pop(int(handle), None)
+    if p is not None:
+        torch.cuda.synchronize(p.ctx.device)  # its tables outlive the queued calls
+        p.close()
+
+
+@torch.library.custom_op("kvexp::prefix_attention", mutates_args=("status",))
+def prefix_attention(k_pages: Tensor, v_pages: Tensor, status: Tensor, q: Tensor, table: Tensor, lens: Tensor,
+                     starts: Tensor | None, prefix: int, scale: float, max_new: int = 0,
+                     max_len: int = 0) -> tuple[Tensor, Tensor]:
+    """PagedCache.attention behind a shared prefix of containers (register_prefix): (out, lse)."""
+    p = _prefixes.get(int(prefix))
+    if p is None:
+        raise ValueError("kvexp.prefix_attention: unknown handle (register_prefix)")
+    cache = _paged(k_pages, v_pages, status)
+    return cache.attention(q, Batch(table, lens, starts, max_new, max_len), scale, p, return_lse=True)
+
+
+@prefix_attention.register_fake
+def _(k_pages, v_pages, status, q, table, lens, starts, prefix, scale, max_new=0, max_len=0):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)

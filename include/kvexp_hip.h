@@ -293,6 +293,137 @@ int kvexp_hip_attention_decode_host(kvexp_hip_ctx *ctx, int order, const uint16_
                                     const uint8_t *v_xkv, size_t v_bytes, float *out, int n_q, int dim, int seq,
                                     int n_threads, int split_tokens);
 
+/* ------------------------------------------------------ paged cache ---- */
+/* A cache of plain keys and values in pages, for batches of sequences: rotary
+ * positions, the append with the rotation on the way, and attention over the
+ * pages and over a prefix that the batch shares. No counterpart in the
+ * reference, which holds one sequence per head and rotates nothing.
+ *
+ * Element type: BF16 or FP16 for pages and rows alike; scores, softmax and sums
+ * are FP32. head_dim is a multiple of 8, at most 256. Pointers of rows and
+ * pages are 16-byte aligned and their strides (in elements) multiples of 8;
+ * the channels of a row are contiguous.
+ *
+ * Calls are stream-ordered, allocate nothing and do not synchronise; their
+ * lengths, tables and positions are read on the device, so a captured call may
+ * be replayed over new ones. Errors that only the device can see (a page
+ * outside the pool, a length past its table, more new tokens than max_new) are
+ * OR-ed into *d_status (required; never cleared by these calls): the rows
+ * concerned are then wrong (a bad page reads page 0, a long length is cut,
+ * nothing is written for a token without a page), the others right, and
+ * nothing outside the given buffers is read or written. */
+enum { KVEXP_HIP_BF16 = 0, KVEXP_HIP_FP16 = 1 };
+#define KVEXP_HIP_STATUS_PAGE 256u   /* a page number outside the pool */
+#define KVEXP_HIP_STATUS_LENGTH 512u /* a length past its table, or more new tokens than max_new */
+
+/* The pool: token t of page p of head h at p * page + h * head + t * token
+ * elements of k and of v. */
+typedef struct kvexp_hip_pages {
+    void *k, *v;
+    int64_t k_page, k_head, k_token;
+    int64_t v_page, v_head, v_token;
+    int32_t dtype, n_pages, page_tokens, n_heads, dim, reserved;
+} kvexp_hip_pages;
+
+/* A batch over the pool (device arrays). Token i of sequence b is token
+ * i % page_tokens of page table[b * table_stride + i / page_tokens]; entries
+ * past lens[b] are not read. Each call brings new tokens, the last ones of
+ * their sequences (counted in lens): rows [starts[b], starts[b + 1]) of its
+ * tensors, or n_tokens / n_seqs rows each where starts is NULL. Rows behind
+ * starts[n_seqs] are left as they are. A sequence with fewer tokens than new
+ * ones has none for the first of them: they are not appended and see nothing.
+ * max_new: the most new tokens of a sequence; max_len: a bound on lens that
+ * the number of splits follows (any value gives right results; <= 0: the
+ * table's). */
+typedef struct kvexp_hip_batch {
+    const int32_t *table;
+    const int32_t *lens;
+    const int32_t *starts; /* n_seqs + 1 entries, or NULL */
+    int64_t table_stride;
+    int32_t table_width, n_seqs, n_tokens, max_new, max_len, reserved;
+} kvexp_hip_batch;
+
+/* Rows [n_tokens, n_heads] of dim channels: data + t * token + h * head. */
+typedef struct kvexp_hip_rows {
+    const void *data;
+    int64_t token, head;
+} kvexp_hip_rows;
+
+/* A rotation of the first 2 n_freq channels: pair i turns by
+ * positions[axes[i]][t] * inv_freq[i] and is scaled by `scale`; pairs are
+ * channels (i, i + n_freq), or (2 i, 2 i + 1) with `interleaved`. axes NULL:
+ * axis 0. Device arrays. */
+typedef struct kvexp_hip_rope {
+    const float *inv_freq; /* [n_freq] */
+    const uint8_t *axes;   /* [n_freq], below n_axes, or NULL */
+    int32_t n_freq, n_axes, interleaved;
+    float scale;
+} kvexp_hip_rope;
+
+/* Positions [n_axes, n_tokens] of the call's tokens, axis_stride elements
+ * apart, int32 or (wide) int64; data NULL: a token's place (its row; its index
+ * in the sequence for an append) plus offset, on every axis. */
+typedef struct kvexp_hip_positions {
+    const void *data;
+    int64_t axis_stride, offset;
+    int32_t wide, reserved;
+} kvexp_hip_positions;
+
+/* Rotates x [n_tokens, n_heads, dim] into out (which may be x). `inverse`
+ * non-zero: the rotation back (the gradient of the rotation). */
+int kvexp_hip_rope_rows(kvexp_hip_ctx *ctx, const kvexp_hip_rope *rope, const kvexp_hip_positions *positions,
+                        const kvexp_hip_rows *x, const kvexp_hip_rows *out, int n_tokens, int n_heads, int dim,
+                        int dtype, int inverse, void *stream);
+
+/* Writes the new tokens' keys (rotated when rope is given) and values
+ * [n_tokens, pages->n_heads, dim] to their pages. With q and q_out the
+ * queries [n_tokens, n_q_heads, dim] are rotated in the same launch. Two
+ * sequences that name the same page and write the same token of it race. */
+int kvexp_hip_paged_append(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, const kvexp_hip_batch *batch,
+                           const kvexp_hip_rows *k, const kvexp_hip_rows *v, const kvexp_hip_rope *rope,
+                           const kvexp_hip_positions *positions, const kvexp_hip_rows *q, const kvexp_hip_rows *q_out,
+                           int n_q_heads, uint32_t *d_status, void *stream);
+
+/* A prefix kept as XKV containers: one K and one V container per KV head, all
+ * of `seq` tokens (as the heads of a plan; n_splits is not used). Reads the
+ * block indexes and builds the tables that the attention kernel needs, ordered
+ * on `stream`, which it synchronises. The containers must not change while it
+ * lives. */
+typedef struct kvexp_hip_prefix kvexp_hip_prefix;
+int kvexp_hip_prefix_create(kvexp_hip_ctx *ctx, const kvexp_hip_head *heads, int n_heads, int dim, void *stream,
+                            kvexp_hip_prefix **out);
+int kvexp_hip_prefix_destroy(kvexp_hip_prefix *prefix);
+
+/* A prefix that every query of the batch sees in front of its sequence: XKV
+ * containers, or the first n_tokens tokens of a table of pages of the pool
+ * (device). */
+typedef struct kvexp_hip_shared {
+    const kvexp_hip_prefix *xkv;
+    const int32_t *table;
+    int32_t table_width, n_tokens;
+} kvexp_hip_shared;
+
+/* Attention of the new tokens' queries q [n_tokens, n_q_heads, dim] over the
+ * pages: token i of a sequence's n new ones sees the first len - n + i + 1
+ * tokens of it (and all of the shared prefix, when given). Query heads
+ * [h g, (h + 1) g) read KV head h, g = n_q_heads / pages->n_heads. out
+ * [n_tokens, n_q_heads, dim] is of the pages' type, d_lse (nullable)
+ * [n_tokens, n_q_heads] FP32 the log of the sum of exponentials. A token that
+ * sees nothing gives 0 and -inf. The workspace (device, 16-byte aligned) holds
+ * at least what kvexp_hip_paged_attention_workspace says for the same
+ * arguments (-1 where they are refused); calls that overlap need one each. */
+int64_t kvexp_hip_paged_attention_workspace(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages,
+                                            const kvexp_hip_batch *batch, const kvexp_hip_shared *shared,
+                                            int n_q_heads);
+int kvexp_hip_paged_attention(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, const kvexp_hip_batch *batch,
+                              const kvexp_hip_shared *shared, const kvexp_hip_rows *q, int n_q_heads, float scale,
+                              const kvexp_hip_rows *out, float *d_lse, void *workspace, size_t workspace_bytes,
+                              uint32_t *d_status, void *stream);
+
+/* Reads and clears a status word of these calls (synchronises `stream`) and
+ * reports what it holds. */
+int kvexp_hip_paged_status(kvexp_hip_ctx *ctx, uint32_t *d_status, void *stream);
+
 /* ------------------------------------------------------------ numerics ---- */
 /* d_y[i] = exp(d_x[i]) with the kernels' exp, which returns the bits of the
  * reference's std::exp(float) (glibc 2.35 expf). No reference counterpart:
