@@ -132,6 +132,24 @@ __device__ __forceinline__ void find_rows(const PagedAttnArgs &a, int seq, int s
     r.t1 = min(r.t0 + r.split_len, seen);
 }
 
+// What a workgroup works on. Consecutive workgroups go to the eight XCDs in
+// turn, so the order decides what shares an XCD and its L2: heads first (they
+// have equal work), then row tiles (the last first, which see the most tokens),
+// then sequences, turned by the split so that the splits of a long sequence, and
+// the first splits, which every sequence has, spread over all of them. (With the
+// splits innermost, 32 or 64 of them: every sequence's split 0 on one XCD, and a
+// draft step of 16 sequences took 97 and 121 us where 48 splits took 63.)
+__device__ __forceinline__ void find_work(const PagedAttnArgs &a, int &split, int &head, int &tile, int &seq) {
+    uint32_t w = blockIdx.x;
+    const uint32_t seqs = a.shared ? 1u : uint32_t(a.batch.n_seqs);
+    head = int(w % uint32_t(a.n_kv));
+    w /= uint32_t(a.n_kv);
+    tile = a.row_tiles - 1 - int(w % uint32_t(a.row_tiles));
+    w /= uint32_t(a.row_tiles);
+    split = int(w / seqs);
+    seq = int((w % seqs + uint32_t(split)) % seqs);
+}
+
 // Tokens that row `row` sees (0 past the rows).
 __device__ __forceinline__ int row_limit(const PagedAttnArgs &a, const Rows &r, int row) {
     if (row >= r.count) return 0;
@@ -187,13 +205,21 @@ __device__ __forceinline__ void write_state(const PagedAttnArgs &a, const Rows &
 }
 
 // --------------------------------------------------------------- few rows --
-// At most 16 query rows per workgroup (a decode step's queries of one KV
-// head): 16 x 16 x 32 products, one per 16 tokens and 32 channels. K and V go
-// from memory to registers, each once: lane (c, g) of a product takes 8
-// channels of token c of K, and of V all its channels (DP / 16 of them) of
-// the 8 tokens 4 g .. 4 g + 3 and 16 + 4 g .., which its own P values belong
-// to; a few byte permutes pair the tokens. The four waves take the split's
-// 32-token tiles in turn and join their states at the end in LDS.
+// Up to 16 NC query rows per workgroup (a decode step's queries of one KV head;
+// a few draft tokens): 16 x 16 x 32 products, one per 16 tokens and 32
+// channels. K and V go from memory to registers, each once: lane (c, g) of a
+// product takes 8 channels of token c of K, and of V all its channels (DP / 16
+// of them) of the 8 tokens 4 g .. 4 g + 3 and 16 + 4 g .., which its own P
+// values belong to; a few byte permutes pair the tokens. The four waves take
+// the split's 32-token tiles in turn and join their states at the end in LDS.
+//
+// Bound: memory. A wave requests its next tile before it works on the one it
+// holds, and the pages of the tile after that: in the first form of this loop
+// every row's address waited for its own table entry, and ten such round trips
+// per tile took 167 us where the loads alone need 60 (64 sequences of 1K to
+// 32K tokens, 2 heads x 7 queries of 64 channels). HALVES: pages of a multiple
+// of 16 tokens, so that 16 tokens share one entry, which then is a scalar; else
+// a lane looks up one token of the tile and the others fetch it from there.
 template <int DP>
 struct Few {
     static constexpr int KS = DP / 32;   // steps of 32 channels
@@ -201,6 +227,26 @@ struct Few {
     static constexpr int VW = C / 2;     // their dwords
     static constexpr int JC = DP > 192 ? DP / 2 : DP; // channels joined at a time (LDS below 64 KiB)
     static constexpr int Row = JC + 4;   // floats per row of the joint state
+    template <bool CAUSAL>
+    static constexpr int Lds = 16 * kPagedWaves * (CAUSAL && DP > Row ? 4 * DP : 4 * Row);
+    // A second tile in registers, and the waves per SIMD that the registers then
+    // allow. More waves hide more than a tile ahead does where both do not fit:
+    // four sequences of up to 65,536 tokens, 8 heads x 4 queries of 128 channels,
+    // 176 us with a tile ahead (two waves), 129 without (three); at 64 channels
+    // both fit three waves (sequences of 1K to 32K: 76 us, 79 with four waves
+    // and no tile ahead). Two products of rows at 128 channels: 75 us with one
+    // wave, 62 with two (16 sequences of up to 8,192, 32 rows).
+    template <int NC>
+    static constexpr bool Ahead = DP <= 64 && NC == 1;
+    // The next tile's K requested as soon as this one's has given its scores,
+    // where the registers hold what that keeps alive (8 queries of 256
+    // channels: 87 -> 80 us; at 128 channels it spills, 118 -> 142).
+    static constexpr bool Early = DP > 192;
+    template <int NC, bool CAUSAL>
+    static constexpr int Occ = NC > 1 ? 2
+                               : DP <= 32 ? 4
+                               : DP <= 128 ? (CAUSAL && DP % 64 == 0 ? 2 : 3)
+                               : DP <= 192 ? 2 : 1;
 };
 
 // N dwords at a 4-byte aligned address.
@@ -229,31 +275,87 @@ struct FewTile {
     uint32_t v[8][Few<DP>::VW];
 };
 
-// Requests the 32 tokens from `tok` (tokens past t1 read token t1 - 1 again).
-template <int DP>
-__device__ __forceinline__ void few_load(const PagedAttnArgs &a, const Rows &r, const int32_t *table,
-                                         const uint16_t *kh, const uint16_t *vh, int tok, int vc,
-                                         FewTile<DP> &f) {
+// Where a tile's tokens lie. HALVES: page and place of tokens 0 and 16 (the
+// same in every lane); else of token lane % 32.
+template <bool HALVES>
+struct FewPlaces;
+template <>
+struct FewPlaces<true> {
+    int page[2], in_page[2];
+};
+template <>
+struct FewPlaces<false> {
+    int page, in_page;
+};
+
+// The table entries of the tile from `tok` (tokens past the last read the
+// last one's).
+template <bool HALVES>
+__device__ __forceinline__ void few_places(const PoolDev &pool, const int32_t *table, int tok, int last,
+                                           FewPlaces<HALVES> &p) {
+    if constexpr (HALVES) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int t = min(tok + 16 * j, last & ~15);
+            const int col = page_of(pool, t);
+            p.in_page[j] = t - col * pool.page_tokens;
+            p.page[j] = table[col];
+        }
+    } else {
+        const int t = min(tok + (lane_id() & 31), last);
+        const int col = page_of(pool, t);
+        p.in_page = t - col * pool.page_tokens;
+        p.page = table[col];
+    }
+}
+
+// A page number held to the pool; `bad` notes the others.
+__device__ __forceinline__ int held_page(const PoolDev &pool, int page, bool &bad) {
+    const bool out = uint32_t(page) >= uint32_t(pool.n_pages);
+    bad |= out;
+    return out ? 0 : page;
+}
+
+// Requests K and V of the tile from `tok` (tokens past `last` are read as tokens
+// that some row sees; what they give is not used). V false: K, and V otherwise.
+template <int DP, bool HALVES, bool V>
+__device__ __forceinline__ void few_load(const PagedAttnArgs &a, const uint16_t *base, int tok, int last, int vc,
+                                         const FewPlaces<HALVES> &p, bool &bad, FewTile<DP> &f) {
     using F = Few<DP>;
     const int lane = lane_id(), c = lane & 15, g = lane >> 4;
-    const int last = r.t1 - 1;
-    int in_page;
+    const int64_t page_step = V ? a.pool.v_page : a.pool.k_page, token_step = V ? a.pool.v_token : a.pool.k_token;
+    auto key = [&](const uint16_t *row, int j) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int page = page_at(a, table, min(tok + 16 * j + c, last), in_page);
-        const uint16_t *row = kh + int64_t(page) * a.pool.k_page + int64_t(in_page) * a.pool.k_token;
+        for (int i = 0; i < F::KS; ++i)
+            f.k[j][i] = *reinterpret_cast<const u32x4a *>(row + min(32 * i + 8 * g, a.dim - 8));
+    };
+    if constexpr (HALVES) {
 #pragma unroll
-        for (int i = 0; i < F::KS; ++i) {
-            const int ch = 32 * i + 8 * g;
-            if (DP % 64 == 0 && a.dim == DP) f.k[j][i] = *reinterpret_cast<const u32x4a *>(row + ch);
-            else f.k[j][i] = ch < a.dim ? *reinterpret_cast<const u32x4a *>(row + ch) : u32x4a{0, 0, 0, 0};
+        for (int j = 0; j < 2; ++j) {
+            const int page = held_page(a.pool, __builtin_amdgcn_readfirstlane(p.page[j]), bad);
+            // the half's tokens: places in_page ..; at the sequence's end the last one again
+            const int room = last - min(tok + 16 * j, last & ~15); // >= 0
+            const uint16_t *at = base + (int64_t(page) * page_step + int64_t(p.in_page[j]) * token_step);
+            if constexpr (!V) key(at + int64_t(min(c, room)) * token_step, j);
+            else {
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                    load_words<F::VW>(at + (int64_t(min(4 * g + n, room)) * token_step + vc), f.v[4 * j + n]);
+            }
         }
-    }
+    } else {
+        const int mine = held_page(a.pool, p.page, bad);
+        auto at = [&](int t) { // the tile's token t
+            const int page = __shfl(mine, t), in = __shfl(p.in_page, t);
+            return base + (int64_t(page) * page_step + int64_t(in) * token_step);
+        };
+        if constexpr (!V) {
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-        const int page = page_at(a, table, min(tok + 4 * g + (n & 3) + 16 * (n >> 2), last), in_page);
-        const uint16_t *row = vh + int64_t(page) * a.pool.v_page + int64_t(in_page) * a.pool.v_token;
-        load_words<F::VW>(row + vc, f.v[n]);
+            for (int j = 0; j < 2; ++j) key(at(16 * j + c), j);
+        } else {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) load_words<F::VW>(at(4 * g + (n & 3) + 16 * (n >> 2)) + vc, f.v[n]);
+        }
     }
 }
 
@@ -267,161 +369,255 @@ __device__ __forceinline__ u32x4a few_v(const FewTile<DP> &f, int jj) {
     return x;
 }
 
-template <int DP, bool HALF>
-__global__ __launch_bounds__(kPagedThreads) void paged_few_kernel(PagedAttnArgs a) {
+template <int DP, bool HALF, int NC, bool HALVES, bool CAUSAL>
+__global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(Few<DP>::template Occ<NC, CAUSAL>, Few<DP>::template Occ<NC, CAUSAL>))) void
+paged_few_kernel(PagedAttnArgs a) {
     using F = Few<DP>;
-    __shared__ float joint[kPagedWaves][16][F::Row];
+    // the waves' states at the end; before, a wave's V of a tile that needs care (below)
+    __shared__ __align__(16) uint8_t lds[F::template Lds<CAUSAL>];
+    float(*joint)[16][F::Row] = reinterpret_cast<float(*)[16][F::Row]>(lds);
     const int lane = lane_id(), c = lane & 15, g = lane >> 4, wave = int(threadIdx.x) >> 6;
-    const int split = int(blockIdx.x), head = int(blockIdx.y) % a.n_kv, tile = int(blockIdx.y) / a.n_kv,
-              seq = int(blockIdx.z);
+    int split, head, tile, seq;
+    find_work(a, split, head, tile, seq);
     Rows r;
-    find_rows(a, seq, split, tile, 16, r);
-    const int r0 = 16 * tile;
+    find_rows(a, seq, split, tile, 16 * NC, r);
+    const int r0 = 16 * NC * tile;
     if (r0 >= r.count || !r.used) return;
-    const int row = r0 + c, limit = row_limit(a, r, row);
     const int low = row_limit(a, r, r0); // the tile's fewest tokens
     const int32_t *table = a.batch.table + (a.shared ? 0 : int64_t(seq) * a.batch.table_stride);
     const uint16_t *kh = a.pool.k + int64_t(head) * a.pool.k_head;
     const uint16_t *vh = a.pool.v + int64_t(head) * a.pool.v_head;
     const int vc = min(F::C * c, a.dim - F::C);
-    // the row's queries: channels 32 i + 8 g ..
-    u32x4a q[F::KS];
-    {
-        const uint16_t *qr = a.q.p + int64_t(row_token(a, r, min(row, r.count - 1))) * a.q.token +
-                             int64_t(head * a.group + min(row, r.count - 1) % a.group) * a.q.head;
+    // the rows' queries: channels 32 i + 8 g ..; rows 16 x + c
+    u32x4a q[NC][F::KS];
+    int limit[NC];
+#pragma unroll
+    for (int x = 0; x < NC; ++x) {
+        const int row = r0 + 16 * x + c, rr = min(row, r.count - 1);
+        limit[x] = row_limit(a, r, row);
+        const uint16_t *qr = a.q.p + int64_t(row_token(a, r, rr)) * a.q.token +
+                             int64_t(head * a.group + rr % a.group) * a.q.head;
 #pragma unroll
         for (int i = 0; i < F::KS; ++i) {
             const int ch = 32 * i + 8 * g;
-            q[i] = row < r.count && ch < a.dim ? *reinterpret_cast<const u32x4a *>(qr + ch) : u32x4a{0, 0, 0, 0};
+            q[x][i] = row < r.count && ch < a.dim ? *reinterpret_cast<const u32x4a *>(qr + ch) : u32x4a{0, 0, 0, 0};
         }
     }
-    f32x4 acc[F::C];
+    f32x4 acc[NC][F::C];
+    float m[NC], l[NC];
 #pragma unroll
-    for (int j = 0; j < F::C; ++j) acc[j] = f32x4{0, 0, 0, 0};
-    float m = -__builtin_inff(), l = 0.0f;
-    for (int tok = r.t0 + 32 * wave; tok < r.t1; tok += 32 * kPagedWaves) {
-        FewTile<DP> f;
-        few_load<DP>(a, r, table, kh, vh, tok, vc, f);
-        f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+    for (int x = 0; x < NC; ++x) {
+        m[x] = -__builtin_inff();
+        l[x] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < F::KS; ++i)
+        for (int j = 0; j < F::C; ++j) acc[x][j] = f32x4{0, 0, 0, 0};
+    }
+    bool bad = false;
+    constexpr int Step = 32 * kPagedWaves;
+    const int last = r.t1 - 1;
+
+    // one tile; once K has given its scores, `keys_done` may request others in its place
+    auto work = [&](FewTile<DP> &f, int tok, auto keys_done) {
+        if (a.dim != DP) { // channels past head_dim: zero, as their queries are
 #pragma unroll
-            for (int j = 0; j < 2; ++j) s[j] = mfma16<HALF>(f.k[j][i], q[i], s[j]);
-        float p[8];
-        const bool cut = tok + 32 > low || tok + 32 > r.t1; // some row does not see some of these tokens
+            for (int i = 0; i < F::KS; ++i)
 #pragma unroll
-        for (int n = 0; n < 8; ++n) p[n] = s[n >> 2][n & 3] * a.scale2;
-        const int seen = min(limit, r.t1) - (tok + 4 * g); // lane's token n is seen if off(n) < seen
-        if (cut) {
-#pragma unroll
-            for (int n = 0; n < 8; ++n)
-                if ((n & 3) + 16 * (n >> 2) >= seen) p[n] = -__builtin_inff();
+                for (int j = 0; j < 2; ++j)
+                    if (32 * i + 8 * g >= a.dim) f.k[j][i] = u32x4a{0, 0, 0, 0};
         }
-        float t = p[0];
-#pragma unroll
-        for (int n = 1; n < 8; ++n) t = fmaxf(t, p[n]);
-        t = fmaxf(t, __shfl_xor(t, 16));
-        t = fmaxf(t, __shfl_xor(t, 32));
-        const float mn = fmaxf(m, t);
-        const float base = mn == -__builtin_inff() ? 0.0f : mn;
-        const float alpha = exp2_f32(m - base);
-        m = mn;
-        l *= alpha;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            p[n] = exp2_f32(p[n] - base);
-            l += p[n];
-        }
-#pragma unroll
-        for (int j = 0; j < F::C; ++j) acc[j] *= alpha;
-        // P as the sum of two 16-bit numbers (16 bits of it, so that an
-        // output's error stays its own rounding; the pass waits for memory)
-        u32x4a hi, lo;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            hi[n] = pack2<HALF>(p[2 * n], p[2 * n + 1]);
-            lo[n] = pack2<HALF>(p[2 * n] - low_f32<HALF>(hi[n]), p[2 * n + 1] - high_f32<HALF>(hi[n]));
-        }
+        const bool cut = tok + 32 > min(low, r.t1); // some row does not see some of these tokens
         bool wild = false;
         if (cut) {
-            bool w = false;
+            if constexpr (CAUSAL) {
+                bool w = false;
 #pragma unroll
-            for (int n = 0; n < 8; ++n)
+                for (int n = 0; n < 8; ++n)
 #pragma unroll
-                for (int k = 0; k < F::VW; ++k) w |= wild2<HALF>(f.v[n][k]);
-            wild = __ballot(w) != 0;
+                    for (int k = 0; k < F::VW; ++k) w |= wild2<HALF>(f.v[n][k]);
+                wild = __ballot(w) != 0;
+            } else { // the rows see the same tokens: the others' values are zero
+#pragma unroll
+                for (int n = 0; n < 8; ++n)
+                    if (tok + 4 * g + (n & 3) + 16 * (n >> 2) >= r.t1)
+#pragma unroll
+                        for (int k = 0; k < F::VW; ++k) f.v[n][k] = 0;
+            }
         }
-        if (!wild) {
+        f32x4 s[NC][2];
+#pragma unroll
+        for (int x = 0; x < NC; ++x) {
+            s[x][0] = s[x][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < F::KS; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) s[x][j] = mfma16<HALF>(f.k[j][i], q[x][i], s[x][j]);
+        }
+        keys_done();
+        u32x4a hi[NC], lo[NC];
+#pragma unroll
+        for (int x = 0; x < NC; ++x) {
+            float p[8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) p[n] = s[x][n >> 2][n & 3] * a.scale2;
+            if (cut) {
+                const int seen = min(limit[x], r.t1) - (tok + 4 * g); // lane's token n is seen if off(n) < seen
+#pragma unroll
+                for (int n = 0; n < 8; ++n)
+                    if ((n & 3) + 16 * (n >> 2) >= seen) p[n] = -__builtin_inff();
+            }
+            float t = p[0];
+#pragma unroll
+            for (int n = 1; n < 8; ++n) t = fmaxf(t, p[n]);
+            t = fmaxf(t, __shfl_xor(t, 16));
+            t = fmaxf(t, __shfl_xor(t, 32));
+            const float mn = fmaxf(m[x], t);
+            const float base = mn == -__builtin_inff() ? 0.0f : mn;
+            const float alpha = exp2_f32(m[x] - base);
+            m[x] = mn;
+            l[x] *= alpha;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                p[n] = exp2_f32(p[n] - base);
+                l[x] += p[n];
+            }
+#pragma unroll
+            for (int j = 0; j < F::C; ++j) acc[x][j] *= alpha;
+            // P as the sum of two 16-bit numbers (16 bits of it, so that an
+            // output's error stays its own rounding; the pass waits for memory)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                hi[x][n] = pack2<HALF>(p[2 * n], p[2 * n + 1]);
+                lo[x][n] = pack2<HALF>(p[2 * n] - low_f32<HALF>(hi[x][n]), p[2 * n + 1] - high_f32<HALF>(hi[x][n]));
+            }
+        }
+        if (!CAUSAL || !wild) {
 #pragma unroll
             for (int j = 0; j < F::C; ++j) {
                 const u32x4a v = few_v<DP>(f, j);
-                acc[j] = mfma16<HALF>(v, hi, acc[j]);
-                acc[j] = mfma16<HALF>(v, lo, acc[j]);
+#pragma unroll
+                for (int x = 0; x < NC; ++x) {
+                    acc[x][j] = mfma16<HALF>(v, hi[x], acc[x][j]);
+                    acc[x][j] = mfma16<HALF>(v, lo[x], acc[x][j]);
+                }
             }
-        } else {
-            // An infinity or NaN among these tokens' V, and rows that do not
-            // see all of them: a token at a time, so that 0 times it stays out
-            // of the rows that do not see it.
-            for (int u = 0; u < 32; ++u) {
-                const int ug = (u >> 2) & 3, un = (u & 3) + 4 * (u >> 4); // its lane group and place there
-                const bool see = tok + u < limit && tok + u < r.t1;
-                const uint32_t keep = g == ug ? (un & 1 ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
-                u32x4a h = u32x4a{0, 0, 0, 0}, w = u32x4a{0, 0, 0, 0};
+            return;
+        }
+        // An infinity or NaN among these tokens' V, and rows that do not see
+        // all of them: a token at a time on the vector ALU, added only where the
+        // row sees it, so that 0 times it stays out of the others.
+        uint32_t *vl = reinterpret_cast<uint32_t *>(lds) + wave * (16 * DP); // V of the tile, a row of DP per token
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int k = 0; k < F::VW; ++k) vl[((4 * g + (n & 3) + 16 * (n >> 2)) * DP + vc) / 2 + k] = f.v[n][k];
+#pragma unroll 1
+        for (int u = 0; u < 32; ++u) { // place un of lane group ug
+            const int ug = (u >> 2) & 3, un = (u & 3) + 4 * (u >> 4);
+#pragma unroll
+            for (int x = 0; x < NC; ++x) {
+                uint32_t h = 0, w = 0;
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
-                    const uint32_t k = n == (un >> 1) ? keep : 0u;
-                    h[n] = hi[n] & k;
-                    w[n] = lo[n] & k;
+                    h = n == (un >> 1) ? hi[x][n] : h;
+                    w = n == (un >> 1) ? lo[x][n] : w;
                 }
+                const float mine = un & 1 ? high_f32<HALF>(h) + high_f32<HALF>(w) : low_f32<HALF>(h) + low_f32<HALF>(w);
+                const float pu = __shfl(mine, c + 16 * ug);
+                if (tok + u >= limit[x] || tok + u >= r.t1) continue;
 #pragma unroll
-                for (int j = 0; j < F::C; ++j) {
-                    u32x4a v = few_v<DP>(f, j);
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) v[n] &= n == (un >> 1) ? keep : 0u;
-                    f32x4 x = mfma16<HALF>(v, h, acc[j]);
-                    x = mfma16<HALF>(v, w, x);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[j][k] = see ? x[k] : acc[j][k];
-                }
+                    for (int k = 0; k < F::VW; ++k) {
+                        const uint32_t v = vl[(u * DP + min(F::C * (4 * g + i), a.dim - F::C)) / 2 + k];
+                        acc[x][2 * k][i] = __builtin_fmaf(pu, low_f32<HALF>(v), acc[x][2 * k][i]);
+                        acc[x][2 * k + 1][i] = __builtin_fmaf(pu, high_f32<HALF>(v), acc[x][2 * k + 1][i]);
+                    }
             }
         }
-    }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    // the waves' states to LDS: lane (c, g) holds row c, channels
-    // min(C (4 g + i), dim - C) + j
-    const int rows = min(16, r.count - r0);
-    if (g == 0) {
-        joint[wave][c][F::JC] = m;
-        joint[wave][c][F::JC + 1] = l;
-    }
-    for (int d0 = 0; d0 < a.dim; d0 += F::JC) {
-        if (d0 > 0) __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int ch = min(F::C * (4 * g + i), a.dim - F::C) - d0;
-#pragma unroll
-            for (int j = 0; j < F::C; ++j)
-                if (F::JC == DP || uint32_t(ch + j) < uint32_t(F::JC)) joint[wave][c][ch + j] = acc[j][i];
-        }
-        __syncthreads();
-        const int nd = min(F::JC, a.dim - d0);
-        for (int i = int(threadIdx.x); i < rows * nd; i += kPagedThreads) {
-            const int rr = i / nd, d = i - rr * nd;
-            float M = -__builtin_inff();
-#pragma unroll
-            for (int w = 0; w < kPagedWaves; ++w) M = fmaxf(M, joint[w][rr][F::JC]);
-            const float base = M == -__builtin_inff() ? 0.0f : M;
-            float L = 0.0f, A = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kPagedWaves; ++w) {
-                const float e = exp2_f32(joint[w][rr][F::JC] - base);
-                // a wave without tokens for the row (l 0) adds nothing
-                const float lw = joint[w][rr][F::JC + 1];
-                L += lw == 0.0f ? 0.0f : lw * e;
-                A += lw == 0.0f ? 0.0f : joint[w][rr][d] * e;
+    };
+
+    int tok = r.t0 + 32 * wave;
+    if (tok < r.t1) {
+        // the places of the tile after the one that is requested are on their way
+        FewPlaces<HALVES> next;
+        FewTile<DP> f0;
+        auto keys = [&](int t, FewTile<DP> &f) { few_load<DP, HALVES, false>(a, kh, t, last, vc, next, bad, f); };
+        auto values = [&](int t, FewTile<DP> &f) { few_load<DP, HALVES, true>(a, vh, t, last, vc, next, bad, f); };
+        auto places = [&](int t) { few_places<HALVES>(a.pool, table, t, last, next); };
+        places(tok);
+        keys(tok, f0);
+        values(tok, f0);
+        places(tok + Step);
+        if constexpr (F::template Ahead<NC>) {
+            FewTile<DP> f1;
+            for (;;) {
+                keys(tok + Step, f1);
+                values(tok + Step, f1);
+                places(tok + 2 * Step);
+                work(f0, tok, [] {});
+                tok += Step;
+                if (tok >= r.t1) break;
+                keys(tok + Step, f0);
+                values(tok + Step, f0);
+                places(tok + 2 * Step);
+                work(f1, tok, [] {});
+                tok += Step;
+                if (tok >= r.t1) break;
             }
-            write_state<HALF>(a, r, head, split, r0 + rr, d0 + d, M, L, A);
+        } else {
+            for (;;) {
+                work(f0, tok, [&] {
+                    if constexpr (F::Early) keys(tok + Step, f0);
+                });
+                tok += Step;
+                if (tok >= r.t1) break;
+                if constexpr (!F::Early) keys(tok, f0);
+                values(tok, f0);
+                places(tok + Step);
+            }
+        }
+        if (bad) atomicOr(a.status, kStPage);
+    }
+    // the waves' states to LDS, 16 rows at a time: lane (c, g) holds row c,
+    // channels min(C (4 g + i), dim - C) + j
+#pragma unroll
+    for (int x = 0; x < NC; ++x) {
+        const int rows = min(16, r.count - r0 - 16 * x);
+        if (rows <= 0) return;
+        l[x] += __shfl_xor(l[x], 16);
+        l[x] += __shfl_xor(l[x], 32);
+        for (int d0 = 0; d0 < a.dim; d0 += F::JC) {
+            __syncthreads(); // (the states before, or a wave's V, are read)
+            if (g == 0 && d0 == 0) {
+                joint[wave][c][F::JC] = m[x];
+                joint[wave][c][F::JC + 1] = l[x];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int ch = min(F::C * (4 * g + i), a.dim - F::C) - d0;
+#pragma unroll
+                for (int j = 0; j < F::C; ++j)
+                    if (F::JC == DP || uint32_t(ch + j) < uint32_t(F::JC)) joint[wave][c][ch + j] = acc[x][j][i];
+            }
+            __syncthreads();
+            const int nd = min(F::JC, a.dim - d0);
+            for (int i = int(threadIdx.x); i < rows * nd; i += kPagedThreads) {
+                const int rr = i / nd, d = i - rr * nd;
+                float M = -__builtin_inff();
+#pragma unroll
+                for (int w = 0; w < kPagedWaves; ++w) M = fmaxf(M, joint[w][rr][F::JC]);
+                const float base = M == -__builtin_inff() ? 0.0f : M;
+                float L = 0.0f, A = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kPagedWaves; ++w) {
+                    const float e = exp2_f32(joint[w][rr][F::JC] - base);
+                    // a wave without tokens for the row (l 0) adds nothing
+                    const float lw = joint[w][rr][F::JC + 1];
+                    L += lw == 0.0f ? 0.0f : lw * e;
+                    A += lw == 0.0f ? 0.0f : joint[w][rr][d] * e;
+                }
+                write_state<HALF>(a, r, head, split, r0 + 16 * x + rr, d0 + d, M, L, A);
+            }
         }
     }
 }
@@ -526,8 +722,8 @@ paged_many_kernel(PagedAttnArgs a) {
     using S = Many<DP>;
     __shared__ ManyLds<DP> lds;
     const int tid = int(threadIdx.x), lane = lane_id(), wave = tid >> 6, c = lane & 31, h = lane >> 5;
-    const int split = int(blockIdx.x), head = int(blockIdx.y) % a.n_kv, tile = int(blockIdx.y) / a.n_kv,
-              seq = int(blockIdx.z);
+    int split, head, tile, seq;
+    find_work(a, split, head, tile, seq);
     Rows r;
     find_rows(a, seq, split, tile, 32 * kPagedWaves, r);
     if (32 * kPagedWaves * tile >= r.count || !r.used) return;

@@ -3,19 +3,49 @@
 #pragma once
 #include "paged_attention.h"
 
+namespace kvexp_dev {
+namespace paged {
+
+inline dim3 attention_grid(const PagedAttnArgs &a, int n_seqs) {
+    return dim3(unsigned(a.n_splits) * unsigned(a.n_kv) * unsigned(a.row_tiles) * unsigned(n_seqs));
+}
+
+template <int DP, bool HALF, int NC, bool HALVES>
+void launch_few_c(const PagedAttnArgs &a, int n_seqs, hipStream_t s) {
+    const dim3 grid = attention_grid(a, n_seqs);
+    // rows of several new tokens see different tokens
+    if (!a.shared && a.batch.max_new > 1)
+        hipLaunchKernelGGL((paged_few_kernel<DP, HALF, NC, HALVES, true>), grid, dim3(kPagedThreads), 0, s, a);
+    else hipLaunchKernelGGL((paged_few_kernel<DP, HALF, NC, HALVES, false>), grid, dim3(kPagedThreads), 0, s, a);
+}
+
+template <int DP, bool HALF>
+void launch_few(const PagedAttnArgs &a, bool two, int n_seqs, hipStream_t s) {
+    const bool halves = a.pool.page_tokens % 16 == 0;
+    if constexpr (kFewRowsAt<DP> == 32)
+        if (two) return halves ? launch_few_c<DP, HALF, 2, true>(a, n_seqs, s) : launch_few_c<DP, HALF, 2, false>(a, n_seqs, s);
+    halves ? launch_few_c<DP, HALF, 1, true>(a, n_seqs, s) : launch_few_c<DP, HALF, 1, false>(a, n_seqs, s);
+}
+
+template <int DP>
+void launch_many(const PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s) {
+    const dim3 grid = attention_grid(a, n_seqs);
+    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kPagedThreads), 0, s, a); };
+    if (a.px != nullptr) run(paged_many_kernel<DP, false, 1>);
+    else if (half) run(paged_many_kernel<DP, true, 0>);
+    else run(paged_many_kernel<DP, false, 0>);
+}
+
+} // namespace paged
+} // namespace kvexp_dev
+
 #define KVEXP_PAGED_LAUNCH(DP)                                                                                        \
-    hipError_t paged_few_d##DP(const kvexp_dev::PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s) {             \
-        using namespace kvexp_dev::paged;                                                                             \
-        const dim3 grid(unsigned(a.n_splits), unsigned(a.n_kv * a.row_tiles), unsigned(n_seqs));                      \
-        if (half) hipLaunchKernelGGL((paged_few_kernel<DP, true>), grid, dim3(kPagedThreads), 0, s, a);               \
-        else hipLaunchKernelGGL((paged_few_kernel<DP, false>), grid, dim3(kPagedThreads), 0, s, a);                   \
+    hipError_t paged_few_d##DP(const kvexp_dev::PagedAttnArgs &a, bool half, bool two, int n_seqs, hipStream_t s) {   \
+        if (half) kvexp_dev::paged::launch_few<DP, true>(a, two, n_seqs, s);                                          \
+        else kvexp_dev::paged::launch_few<DP, false>(a, two, n_seqs, s);                                              \
         return hipGetLastError();                                                                                     \
     }                                                                                                                 \
     hipError_t paged_many_d##DP(const kvexp_dev::PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s) {            \
-        using namespace kvexp_dev::paged;                                                                             \
-        const dim3 grid(unsigned(a.n_splits), unsigned(a.n_kv * a.row_tiles), unsigned(n_seqs));                      \
-        if (a.px != nullptr) hipLaunchKernelGGL((paged_many_kernel<DP, false, 1>), grid, dim3(kPagedThreads), 0, s, a); \
-        else if (half) hipLaunchKernelGGL((paged_many_kernel<DP, true, 0>), grid, dim3(kPagedThreads), 0, s, a);      \
-        else hipLaunchKernelGGL((paged_many_kernel<DP, false, 0>), grid, dim3(kPagedThreads), 0, s, a);               \
+        kvexp_dev::paged::launch_many<DP>(a, half, n_seqs, s);                                                        \
         return hipGetLastError();                                                                                     \
     }

@@ -8,9 +8,11 @@ namespace kvexp_dev {
 namespace paged {
 namespace {
 
-// Joins the states of a row: maximum, then the weighted sums. One wave per
-// row; lane s takes the weight of split s of a batch of 64, then every lane
-// its channels of the batch's rows, in split order (the same sum every time).
+// Joins the states of a row: maximum, then the weighted sums. W waves per row,
+// wave w the splits w, w + W, ..; lane i takes the weight of its wave's i-th
+// split of a batch of 64, then every lane its channels of the batch's rows, in
+// split order (the same sum every time). Every row's sums are read, four in
+// flight: a split that saw nothing of the row has weight 0 and sums 0.
 struct Joined {
     float m = -__builtin_inff(), l = 0.0f;
     float acc[4] = {0, 0, 0, 0};
@@ -25,14 +27,27 @@ __device__ __forceinline__ float wave_sum_all(float x) {
     return x;
 }
 
-__device__ __forceinline__ void join(Joined &j, const float *acc, const float *ml, int64_t slot, int64_t step, int n,
-                                     int dim) {
+template <int CH> // channels per lane
+__device__ __forceinline__ void join_rows(Joined &j, const float *acc, int64_t step, int cnt, float w, int dim) {
     const int lane = lane_id();
-    for (int s0 = 0; s0 < n; s0 += kWave) {
-        const int cnt = min(kWave, n - s0);
+#pragma unroll 8
+    for (int i = 0; i < cnt; ++i) {
+        const float wi = readlane_f32(w, i);
+        const float *row = acc + i * step;
+#pragma unroll
+        for (int k = 0; k < CH; ++k) j.acc[k] = __builtin_fmaf(wi, row[min(lane + kWave * k, dim - 1)], j.acc[k]);
+    }
+}
+
+// Splits first, first + every, .. below n of the row whose split 0 is in `slot`.
+__device__ __forceinline__ void join(Joined &j, const float *acc, const float *ml, int64_t slot, int64_t step, int first,
+                                     int every, int n, int dim) {
+    const int lane = lane_id(), mine = first < n ? (n - first + every - 1) / every : 0;
+    for (int s0 = 0; s0 < mine; s0 += kWave) {
+        const int cnt = min(kWave, mine - s0);
         float m = -__builtin_inff(), l = 0.0f;
         if (lane < cnt) {
-            const float2 x = *reinterpret_cast<const float2 *>(ml + 2 * (slot + (s0 + lane) * step));
+            const float2 x = *reinterpret_cast<const float2 *>(ml + 2 * (slot + (first + (s0 + lane) * every) * step));
             m = x.x;
             l = x.y;
         }
@@ -43,17 +58,10 @@ __device__ __forceinline__ void join(Joined &j, const float *acc, const float *m
         j.l = j.l * old + wave_sum_all(l == 0.0f ? 0.0f : w * l);
 #pragma unroll
         for (int k = 0; k < 4; ++k) j.acc[k] *= old;
-#pragma unroll 4
-        for (int i = 0; i < cnt; ++i) {
-            const float wi = readlane_f32(w, i), li = readlane_f32(l, i);
-            if (li == 0.0f) continue; // nothing there (its sums were not written)
-            const float *row = acc + (slot + (s0 + i) * step) * dim;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int d = lane + kWave * k;
-                if (d < dim) j.acc[k] = __builtin_fmaf(wi, row[d], j.acc[k]);
-            }
-        }
+        const float *rows = acc + (slot + int64_t(first + s0 * every) * step) * dim;
+        if (dim <= 64) join_rows<1>(j, rows, every * step * dim, cnt, w, dim);
+        else if (dim <= 128) join_rows<2>(j, rows, every * step * dim, cnt, w, dim);
+        else join_rows<4>(j, rows, every * step * dim, cnt, w, dim);
     }
 }
 
@@ -89,29 +97,53 @@ __global__ __launch_bounds__(256) void prefix_segs_kernel(PrefixSeg *__restrict_
     segs[i] = s;
 }
 
-template <bool HALF>
+template <bool HALF, int W>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a, int rows_per_seq) {
+    __shared__ float part[4][kMaxDim + 2];
     const int hq_all = a.n_kv * a.group;
-    const int64_t w = int64_t(blockIdx.x) * 4 + (int(threadIdx.x) >> 6);
-    const int seq = int(w / rows_per_seq);
+    const int wave = int(threadIdx.x) >> 6, lane = lane_id();
+    const int64_t at = W == 4 ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * 4 + wave;
+    const int seq = int(at / rows_per_seq);
     if (seq >= a.batch.n_seqs) return;
-    const int rest = int(w - int64_t(seq) * rows_per_seq);
+    const int rest = int(at - int64_t(seq) * rows_per_seq);
     const int i = rest / hq_all, hq = rest - i * hq_all;
     Rows r;
     find_rows(a, seq, 1, 1, 1, r); // (split and tile 1: no errors raised here)
     if (i >= r.n) return;
     const int head = hq / a.group, g = hq - head * a.group;
-    const int row = i * a.group + g;
     const int64_t tok = r.first + i;
+    const int first = W == 4 ? wave : 0;
     Joined j;
     if (a.s_splits > 0) {
         const int len = split_tokens(a.s_len, a.s_splits, a.s_min_split);
         const int n = max(1, (a.s_len + len - 1) / len);
-        join(j, a.s_acc, a.s_ml, int64_t(head) * a.s_splits * a.s_rows + tok * a.group + g, a.s_rows, n, a.dim);
+        join(j, a.s_acc, a.s_ml, int64_t(head) * a.s_splits * a.s_rows + tok * a.group + g, a.s_rows, first, W, n, a.dim);
     }
     const int n = max(1, (r.len + r.split_len - 1) / r.split_len);
-    join(j, a.acc, a.ml, state_slot(a, r, head, 0, row), a.max_rows, n, a.dim);
-    const int lane = lane_id();
+    join(j, a.acc, a.ml, state_slot(a, r, head, 0, i * a.group + g), a.max_rows, first, W, n, a.dim);
+    if constexpr (W == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) part[wave][lane + kWave * k] = j.acc[k];
+        if (lane == 0) {
+            part[wave][kMaxDim] = j.m;
+            part[wave][kMaxDim + 1] = j.l;
+        }
+        __syncthreads();
+        if (wave != 0) return;
+        float M = -__builtin_inff();
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, part[w][kMaxDim]);
+        const float base = M == -__builtin_inff() ? 0.0f : M;
+        j = Joined{};
+        j.m = M;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float l = part[w][kMaxDim + 1], e = l == 0.0f ? 0.0f : exp2_f32(part[w][kMaxDim] - base);
+            j.l += l == 0.0f ? 0.0f : e * l;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) j.acc[k] = __builtin_fmaf(e, part[w][lane + kWave * k], j.acc[k]);
+        }
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int d = lane + kWave * k;
@@ -129,7 +161,7 @@ namespace kvexp_launch {
 using namespace kvexp_dev;
 
 #define KVEXP_PAGED_DECL(DP)                                                                       \
-    hipError_t paged_few_d##DP(const PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s);      \
+    hipError_t paged_few_d##DP(const PagedAttnArgs &a, bool half, bool two, int n_seqs, hipStream_t s); \
     hipError_t paged_many_d##DP(const PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s);
 KVEXP_PAGED_DECL(32)
 KVEXP_PAGED_DECL(64)
@@ -138,9 +170,11 @@ KVEXP_PAGED_DECL(128)
 KVEXP_PAGED_DECL(192)
 KVEXP_PAGED_DECL(256)
 
-hipError_t paged_attention(const PagedAttnArgs &a, bool half, bool many, int n_seqs, hipStream_t s) {
+// tile_rows: 16 or 32 (the few-row kernel), or the many-row kernel's.
+hipError_t paged_attention(const PagedAttnArgs &a, bool half, int tile_rows, int n_seqs, hipStream_t s) {
+    const bool many = tile_rows > 32, two = tile_rows == 32;
 #define KVEXP_PAGED_PICK(DP) \
-    if (a.dim <= DP) return many ? paged_many_d##DP(a, half, n_seqs, s) : paged_few_d##DP(a, half, n_seqs, s);
+    if (a.dim <= DP) return many ? paged_many_d##DP(a, half, n_seqs, s) : paged_few_d##DP(a, half, two, n_seqs, s);
     KVEXP_PAGED_PICK(32)
     KVEXP_PAGED_PICK(64)
     KVEXP_PAGED_PICK(96)
@@ -157,10 +191,15 @@ hipError_t prefix_segs(PrefixSeg *segs, int n, const EscJob *jobs, hipStream_t s
 
 hipError_t paged_merge(const PagedAttnArgs &a, bool half, hipStream_t s) {
     const int rows = a.batch.max_new * a.n_kv * a.group;
-    const int64_t waves = int64_t(a.batch.n_seqs) * rows;
-    const dim3 grid(unsigned((waves + 3) / 4));
-    if (half) hipLaunchKernelGGL(paged::paged_merge_kernel<true>, grid, dim3(256), 0, s, a, rows);
-    else hipLaunchKernelGGL(paged::paged_merge_kernel<false>, grid, dim3(256), 0, s, a, rows);
+    const int64_t n = int64_t(a.batch.n_seqs) * rows;
+    // four waves per row where the rows alone do not fill the GPU and there
+    // are splits for them
+    const bool four = n < 4096 && a.n_splits + a.s_splits >= 8;
+    auto run = [&](auto kernel, int64_t groups) {
+        hipLaunchKernelGGL(kernel, dim3(unsigned(groups)), dim3(256), 0, s, a, rows);
+    };
+    if (four) half ? run(paged::paged_merge_kernel<true, 4>, n) : run(paged::paged_merge_kernel<false, 4>, n);
+    else half ? run(paged::paged_merge_kernel<true, 1>, (n + 3) / 4) : run(paged::paged_merge_kernel<false, 1>, (n + 3) / 4);
     return hipGetLastError();
 }
 

@@ -120,5 +120,10 @@ struct PagedAttnArgs {
 
 // Tokens of a tile of the many-row kernel.
 constexpr int tile_tokens(int dim) { return dim <= 128 ? 64 : 32; }
+// Query rows of a workgroup of the few-row kernel, at most: 16, or 32 in two
+// products where the registers hold them.
+constexpr int few_rows(int dim) { return dim <= 128 ? 32 : 16; }
+template <int DP>
+constexpr int kFewRowsAt = few_rows(DP);
 
 } // namespace kvexp_dev

@@ -15,7 +15,7 @@ using namespace kvexp_dev;
 
 namespace kvexp_launch {
 hipError_t rotate(RotateArgs a, bool half, hipStream_t s);
-hipError_t paged_attention(const PagedAttnArgs &a, bool half, bool many, int n_seqs, hipStream_t s);
+hipError_t paged_attention(const PagedAttnArgs &a, bool half, int tile_rows, int n_seqs, hipStream_t s);
 hipError_t paged_merge(const PagedAttnArgs &a, bool half, hipStream_t s);
 hipError_t prefix_segs(PrefixSeg *segs, int n, const EscJob *jobs, hipStream_t s);
 } // namespace kvexp_launch
@@ -30,8 +30,8 @@ struct kvexp_hip_prefix {
 namespace {
 
 constexpr int kMaxHeadDim = 256;
-constexpr int kGridMax = 65535;
-constexpr int kFewRows = 16, kManyRows = 128;
+constexpr int64_t kGridMax = (int64_t(1) << 24) - 1; // workgroups of 256 threads below 2^32 threads
+constexpr int kManyRows = 128;
 
 [[noreturn]] void bad(const std::string &msg) { fail(KVEXP_HIP_INVALID_ARGUMENT, msg); }
 
@@ -149,24 +149,26 @@ RopeDev rope_of(const char *who, const kvexp_hip_rope *r, const kvexp_hip_positi
 
 // How a call is cut.
 struct Cut {
-    bool many = false;
-    int row_tiles = 1, n_splits = 1, min_split = 64, rows = 0;
+    int tile_rows = 16, row_tiles = 1, n_splits = 1, min_split = 64, rows = 0;
 };
 
-// Rows per (sequence, head) pick the kernel: up to 16 fill one product of the
-// few-row kernel, more take the many-row kernel, whose tiles go through LDS.
-Cut cut_of(const kvexp_hip_ctx *ctx, int64_t rows, int64_t pairs, int max_len, bool coded) {
+// Rows per (sequence, head) pick the kernel: what a workgroup of the few-row
+// kernel takes (few_rows), or the many-row kernel, whose tiles go through LDS.
+Cut cut_of(const kvexp_hip_ctx *ctx, int64_t rows, int64_t pairs, int max_len, int dim, bool coded) {
     Cut c;
     if (rows > INT32_MAX / 2) fail(KVEXP_HIP_UNSUPPORTED, "paged attention: too many query rows");
     c.rows = int(rows);
-    c.many = coded || rows > kFewRows;
-    const int per = c.many ? kManyRows : kFewRows;
-    c.row_tiles = int((rows + per - 1) / per);
+    const bool many = coded || rows > few_rows(dim);
+    c.tile_rows = many ? kManyRows : rows > 16 ? 32 : 16;
+    c.row_tiles = int((rows + c.tile_rows - 1) / c.tile_rows);
     c.min_split = 256;
-    const int64_t target = int64_t(std::max(1, ctx->cu_count)) * (c.many ? 2 : 16);
+    const int64_t target = int64_t(std::max(1, ctx->cu_count)) * (many ? 2 : 8);
     const int64_t base = std::max<int64_t>(1, pairs * c.row_tiles);
     const int64_t most = std::max<int64_t>(1, (int64_t(max_len) + c.min_split - 1) / c.min_split);
     c.n_splits = int(std::max<int64_t>(1, std::min<int64_t>({(target + base - 1) / base, most, 256})));
+    // the splits of the longest sequence the call may hold: shorter ones take fewer
+    const int64_t even = (int64_t(max_len) + c.n_splits - 1) / c.n_splits;
+    c.min_split = int(std::max<int64_t>(c.min_split, (even + 63) / 64 * 64));
     return c;
 }
 
@@ -214,8 +216,8 @@ Call plan_call(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, const kvexp_hip
     if (c.has_shared && shared->xkv != nullptr && shared->xkv->ctx->device != ctx->device)
         bad(std::string(who) + ": the prefix is on another device");
     const int64_t rows = int64_t(a.batch.max_new) * a.group;
-    c.cut = cut_of(ctx, rows, int64_t(a.batch.n_seqs) * a.n_kv, max_len, false);
-    if (a.batch.n_seqs > kGridMax || int64_t(a.n_kv) * c.cut.row_tiles > kGridMax ||
+    c.cut = cut_of(ctx, rows, int64_t(a.batch.n_seqs) * a.n_kv, max_len, a.dim, false);
+    if (int64_t(a.batch.n_seqs) * a.n_kv * c.cut.row_tiles * c.cut.n_splits > kGridMax ||
         int64_t(a.batch.n_seqs) * a.batch.max_new * n_q_heads > INT32_MAX)
         fail(KVEXP_HIP_UNSUPPORTED, std::string(who) + ": more sequences or query rows than a launch takes");
     a.row_tiles = c.cut.row_tiles;
@@ -235,8 +237,8 @@ Call plan_call(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, const kvexp_hip
         p.direct = 0;
         p.len = shared->n_tokens;
         const bool xkv = shared->xkv != nullptr;
-        c.shared_cut = cut_of(ctx, int64_t(a.batch.n_tokens) * a.group, a.n_kv, p.len, xkv);
-        if (int64_t(a.n_kv) * c.shared_cut.row_tiles > kGridMax)
+        c.shared_cut = cut_of(ctx, int64_t(a.batch.n_tokens) * a.group, a.n_kv, p.len, a.dim, xkv);
+        if (int64_t(a.n_kv) * c.shared_cut.row_tiles * c.shared_cut.n_splits > kGridMax)
             fail(KVEXP_HIP_UNSUPPORTED, std::string(who) + ": more query rows than a launch takes");
         p.row_tiles = c.shared_cut.row_tiles;
         p.n_splits = c.shared_cut.n_splits;
@@ -537,9 +539,9 @@ int kvexp_hip_paged_attention(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, 
             p.ml = reinterpret_cast<float *>(w + c.at_shared_ml);
             a.s_acc = p.acc;
             a.s_ml = p.ml;
-            HIPX(kvexp_launch::paged_attention(p, c.half, c.shared_cut.many, 1, s));
+            HIPX(kvexp_launch::paged_attention(p, c.half, c.shared_cut.tile_rows, 1, s));
         }
-        HIPX(kvexp_launch::paged_attention(a, c.half, c.cut.many, a.batch.n_seqs, s));
+        HIPX(kvexp_launch::paged_attention(a, c.half, c.cut.tile_rows, a.batch.n_seqs, s));
         if (!a.direct) HIPX(kvexp_launch::paged_merge(a, c.half, s));
     });
 }
