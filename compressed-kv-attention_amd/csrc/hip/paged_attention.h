@@ -16,6 +16,7 @@
 // the tokens of its operand; V is read in the same order).
 #pragma once
 
+#include "attention_team.h"
 #include "paged_device.h"
 
 #include <hip/hip_fp16.h>
@@ -632,6 +633,17 @@ paged_few_kernel(PagedAttnArgs a) {
 // the second product would else cost twice, and the error that this leaves in
 // an output (a sum of independent roundings) is as large as the output's own
 // rounding.
+//
+// Bound: the vector ALU (per tile and wave 32 exponentials at a quarter of its
+// rate, their arguments, maxima and sums) and the matrix cores, in turn. The
+// tile after next is on its way in registers and the next one in the other
+// half of LDS while a tile is worked on; a workgroup's waves meet once per tile
+// (containers: twice, the escapes being written over their elements between),
+// and two workgroups share a CU, so that one's products run beside the other's
+// exponentials.
+#ifndef XUNR
+#define XUNR 1
+#endif
 template <int DP>
 struct Many {
     static constexpr int KT = tile_tokens(DP);
@@ -641,16 +653,23 @@ struct Many {
     static constexpr int KR = DP + 8;                         // LDS elements per row of K: rows 4 banks apart
     static constexpr int VR = DP + (DP % 64 == 0 ? 32 : 0);   // of V: four rows 16 banks apart
     static constexpr int PR = DP / 8;                         // 16-byte pieces per row
-    static constexpr int Occ = DP <= 96 ? 2 : 1;              // waves per SIMD that the registers allow
-    static constexpr int NP = KT * PR / kPagedThreads;        // pieces per thread
+    static constexpr int Occ = DP <= 128 ? 2 : 1;             // waves per SIMD that the registers allow
+    static constexpr int NP = KT * PR / kPagedThreads;        // pieces per thread (pages)
     static_assert(KT * PR % kPagedThreads == 0, "whole pieces per thread");
+    // containers: a thread keeps to one column of 8 channels, RP rows a pass
+    static constexpr int RP = kPagedThreads / PR;
+    static constexpr int NR = (KT + RP - 1) / RP;
 };
 
 template <int DP>
-struct alignas(16) ManyLds {
+struct alignas(16) ManyBuf {
     uint16_t k[Many<DP>::KT * Many<DP>::KR];
     uint16_t v[Many<DP>::KT * Many<DP>::VR];
-    int2 row[Many<DP>::KT]; // page and place of the next tile's tokens
+};
+template <int DP>
+struct alignas(16) ManyLds {
+    ManyBuf<DP> buf[2];
+    int2 row[2][Many<DP>::KT]; // page and place of the tokens of tiles on their way
 };
 
 typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
@@ -658,61 +677,150 @@ typedef uint32_t any_u32x2 __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t any_u32 __attribute__((aligned(1)));
 typedef uint16_t any_u16 __attribute__((aligned(1)));
 
-// Two elements of a coded row: bytes b and b + 1 of sm and of base, with their codes.
-__device__ __forceinline__ uint32_t join_pair(uint32_t sm, uint32_t base, int b, uint32_t c0, uint32_t c1) {
-    return bf16_join(((base >> (8 * b)) & 0xFFu) + c0, (sm >> (8 * b)) & 0xFFu) |
-           (bf16_join(((base >> (8 * b + 8)) & 0xFFu) + c1, (sm >> (8 * b + 8)) & 0xFFu) << 16);
-}
+// An octet of channels of a coded tensor is kept in LDS as the decoder of the
+// decode kernels gives it: dword p holds channels p and p + 4. The queries are
+// put in the same order, and the outputs back from it.
+__device__ __forceinline__ int octet_place(int ch) { return (ch & ~7) | ((ch & 3) << 1) | ((ch >> 2) & 1); }
 
-// Eight channels from channel `ch` of row `row` of a segment (escapes come after).
-__device__ __forceinline__ u32x4a seg_octet(const PrefixSeg &s, int dim, int row, int ch) {
+// 8 channels of one row of a run, as they lie in the container.
+struct CodedOctet {
+    uint2 sm; // sign/mantissa bytes (a plain block: the first 8 bytes)
+    uint2 c;  // x: the codes (a plain block: the other 8 bytes)
+};
+
+// The octet from channel ch of row `row` of a run.
+__device__ __forceinline__ void load_octet(const PrefixSeg &s, int dim, int row, int ch, CodedOctet &o) {
     const int e = (s.row0 + row) * dim + ch; // element of the block
-    if (s.mode == 0) {
-        const any_u32x4 v = *reinterpret_cast<const any_u32x4 *>(s.data + 2 * e);
-        return u32x4a{v.x, v.y, v.z, v.w};
-    }
-    const any_u32x2 base = *reinterpret_cast<const any_u32x2 *>(s.data + ch);
-    const any_u32x2 sm = *reinterpret_cast<const any_u32x2 *>(s.data + dim + e);
+    const uint8_t *p = s.mode == 0 ? s.data + 2 * e : s.data + dim + e;
+    const any_u32x2 sm = *reinterpret_cast<const any_u32x2 *>(p);
+    o.sm = make_uint2(sm.x, sm.y);
     const uint8_t *cp = s.data + dim + s.n_tokens * dim + (e >> 3) * s.mode;
-    uint32_t c;
-    if (s.mode == 4) c = *reinterpret_cast<const any_u32 *>(cp);
-    else if (s.mode == 2) c = *reinterpret_cast<const any_u16 *>(cp);
-    else c = uint32_t(cp[0]) | (uint32_t(cp[1]) << 8) | (uint32_t(cp[2]) << 16);
-    const uint32_t mask = (1u << s.mode) - 1u;
-    auto code = [&](int i) { return (c >> (s.mode * i)) & mask; };
-    return u32x4a{join_pair(sm.x, base.x, 0, code(0), code(1)), join_pair(sm.x, base.x, 2, code(2), code(3)),
-                  join_pair(sm.y, base.y, 0, code(4), code(5)), join_pair(sm.y, base.y, 2, code(6), code(7))};
+    if (s.mode == 4) o.c.x = *reinterpret_cast<const any_u32 *>(cp);
+    else if (s.mode == 2) o.c.x = *reinterpret_cast<const any_u16 *>(cp);
+    else if (s.mode == 3) o.c.x = uint32_t(*reinterpret_cast<const any_u16 *>(cp)) | (uint32_t(cp[2]) << 16);
+    else {
+        const any_u32x2 x = *reinterpret_cast<const any_u32x2 *>(p + 8);
+        o.c = make_uint2(x.x, x.y);
+    }
 }
 
-// A tile of a container tensor to LDS rows of R elements; V: rows past the
-// tile's tokens are zero.
-template <int R, int KT, bool V>
-__device__ __forceinline__ void stage_coded(const PrefixTensor &t, int tile, int dim, int rows, uint16_t *lds) {
-    const int pr = dim / 8;
-    for (int s = t.tile_seg[tile]; s < t.tile_seg[tile + 1]; ++s) {
-        const PrefixSeg seg = t.segs[s];
-        for (int o = int(threadIdx.x); o < seg.rows * pr; o += kPagedThreads) {
-            const int row = o / pr, ch = 8 * (o - row * pr);
-            *reinterpret_cast<u32x4a *>(lds + (seg.dst + row) * R + ch) = seg_octet(seg, dim, row, ch);
+// The octet's BF16 words in octet order (escapes come after), from its base
+// words (channels p and p + 4 of the block's base exponents, shifted by 7).
+template <int MODE>
+__device__ __forceinline__ u32x4a decode_octet(const CodedOctet &o, const uint32_t (&bp)[4], uint32_t smm) {
+    uint32_t cw, t[4];
+    if constexpr (MODE == 4) cw = o.c.x;
+    else if constexpr (MODE == 2) cw = __builtin_amdgcn_perm(o.c.x, o.c.x, 0x0c010c00u);
+    else cw = (o.c.x & 0xFFFu) | ((o.c.x << 4) & 0x0FFF0000u);
+    team::octet_exponents<MODE>(cw, bp, t);
+    return u32x4a{team::team_pair(o.sm.x, o.sm.y, 0, t[0], smm), team::team_pair(o.sm.x, o.sm.y, 1, t[1], smm),
+                  team::team_pair(o.sm.x, o.sm.y, 2, t[2], smm), team::team_pair(o.sm.x, o.sm.y, 3, t[3], smm)};
+}
+__device__ __forceinline__ u32x4a plain_octet(const CodedOctet &o) {
+    const uint4 x = team::raw_octet(make_uint4(o.sm.x, o.sm.y, o.c.x, o.c.y));
+    return u32x4a{x.x, x.y, x.z, x.w};
+}
+__device__ __forceinline__ void base_words(uint2 base, uint32_t (&bp)[4]) {
+#pragma unroll
+    for (uint32_t p = 0; p < 4; ++p)
+        bp[p] = __builtin_amdgcn_perm(base.y, base.x, 0x0c000c00u | ((4u + p) << 16) | p) << 7;
+}
+
+// A tile of a container tensor on its way: the rows of its first run in
+// registers (pass k: row RP k + the thread's row), and its first escape
+// records, one per thread.
+template <int DP>
+struct CodedTile {
+    CodedOctet o[Many<DP>::NR];
+    uint2 base;
+    uint32_t rec;
+};
+
+// The thread's column and row of a pass; rows per pass.
+struct Column {
+    int ch, row, step;
+};
+
+template <int DP>
+__device__ __forceinline__ void coded_load(const PrefixSeg &s, int dim, const Column &at, CodedTile<DP> &t) {
+    const int tid = int(threadIdx.x);
+    t.rec = s.esc[max(min(tid, s.n_esc - 1), 0)];
+    const int lastp = s.rows - 1;
+    if (s.mode != 0) {
+        const any_u32x2 b = *reinterpret_cast<const any_u32x2 *>(s.data + at.ch);
+        t.base = make_uint2(b.x, b.y);
+    }
+#pragma unroll
+    for (int k = 0; k < Many<DP>::NR; ++k) load_octet(s, dim, min(at.row + at.step * k, lastp), at.ch, t.o[k]);
+}
+
+// The run's rows to LDS rows of R elements; V: the tile's other rows are zero
+// (a run of the tile's end: the prefix's end) before further runs are written.
+template <int DP, int R, bool V>
+__device__ __forceinline__ void coded_store(const PrefixSeg &s, const PrefixSeg *segs, int dim, const Column &at,
+                                            const CodedTile<DP> &t, uint16_t *lds) {
+    using S = Many<DP>;
+    const uint32_t smm = wave::sm_mask_vgpr();
+    const bool mine = at.row < at.step; // (threads past the whole rows of a pass have none)
+    auto put = [&](auto octet) {
+#pragma unroll
+        for (int k = 0; k < S::NR; ++k) {
+            const int row = at.row + at.step * k;
+            const u32x4a w = octet(k);
+            if (mine && row < s.rows) *reinterpret_cast<u32x4a *>(lds + row * R + at.ch) = w;
+            else if (V && mine && row < S::KT && s.n_more == 0)
+                *reinterpret_cast<u32x4a *>(lds + row * R + at.ch) = u32x4a{0, 0, 0, 0};
+        }
+    };
+    uint32_t bp[4];
+    base_words(t.base, bp);
+    if (s.mode == 4) put([&](int k) { return decode_octet<4>(t.o[k], bp, smm); });
+    else if (s.mode == 2) put([&](int k) { return decode_octet<2>(t.o[k], bp, smm); });
+    else if (s.mode == 3) put([&](int k) { return decode_octet<3>(t.o[k], bp, smm); });
+    else put([&](int k) { return plain_octet(t.o[k]); });
+    if (s.n_more == 0) return;
+    // blocks that end inside the tile: their rows are read here
+    int end = s.rows;
+    for (int i = 0; i < s.n_more; ++i) {
+        const PrefixSeg g = segs[s.more + i];
+        end = g.dst + g.rows;
+        uint2 base = make_uint2(0, 0);
+        if (g.mode != 0) {
+            const any_u32x2 b = *reinterpret_cast<const any_u32x2 *>(g.data + at.ch);
+            base = make_uint2(b.x, b.y);
+        }
+        base_words(base, bp);
+        for (int row = at.row; mine && row < g.rows; row += at.step) {
+            CodedOctet o;
+            load_octet(g, dim, row, at.ch, o);
+            *reinterpret_cast<u32x4a *>(lds + (g.dst + row) * R + at.ch) =
+                g.mode == 4   ? decode_octet<4>(o, bp, smm)
+                : g.mode == 2 ? decode_octet<2>(o, bp, smm)
+                : g.mode == 3 ? decode_octet<3>(o, bp, smm)
+                              : plain_octet(o);
         }
     }
     if (V)
-        for (int o = rows * pr + int(threadIdx.x); o < KT * pr; o += kPagedThreads) {
-            const int row = o / pr, ch = 8 * (o - row * pr);
-            *reinterpret_cast<u32x4a *>(lds + row * R + ch) = u32x4a{0, 0, 0, 0};
-        }
+        for (int row = end + at.row; mine && row < S::KT; row += at.step)
+            *reinterpret_cast<u32x4a *>(lds + row * R + at.ch) = u32x4a{0, 0, 0, 0};
 }
-// The tile's escapes over their elements.
+
+// An escape record of a run over its element.
 template <int R>
-__device__ __forceinline__ void patch_coded(const PrefixTensor &t, int tile, int dim, uint16_t *lds) {
-    for (int s = t.tile_seg[tile]; s < t.tile_seg[tile + 1]; ++s) {
-        const PrefixSeg seg = t.segs[s];
-        for (int i = int(threadIdx.x); i < seg.n_esc; i += kPagedThreads) {
-            const uint32_t rec = seg.esc[i];
-            const int e = int(rec & 0xFFFFu), row = e / dim - seg.row0;
-            if (uint32_t(row) < uint32_t(seg.rows)) // (a damaged container's records)
-                lds[(seg.dst + row) * R + (e - (row + seg.row0) * dim)] = uint16_t(rec >> 16);
-        }
+__device__ __forceinline__ void patch_one(const PrefixSeg &s, int dim, uint32_t rec, uint16_t *lds) {
+    const int e = int(rec & 0xFFFFu), row = e / dim - s.row0;
+    if (uint32_t(row) < uint32_t(s.rows)) // (a damaged container's records)
+        lds[(s.dst + row) * R + octet_place(e - (row + s.row0) * dim)] = uint16_t(rec >> 16);
+}
+template <int DP, int R>
+__device__ __forceinline__ void coded_patch(const PrefixSeg &s, const PrefixSeg *segs, int dim, const CodedTile<DP> &t,
+                                            uint16_t *lds) {
+    const int tid = int(threadIdx.x);
+    if (tid < s.n_esc) patch_one<R>(s, dim, t.rec, lds);
+    for (int i = tid + kPagedThreads; i < s.n_esc; i += kPagedThreads) patch_one<R>(s, dim, s.esc[i], lds);
+    for (int k = 0; k < s.n_more; ++k) {
+        const PrefixSeg g = segs[s.more + k];
+        for (int i = tid; i < g.n_esc; i += kPagedThreads) patch_one<R>(g, dim, g.esc[i], lds);
     }
 }
 
@@ -720,7 +828,8 @@ template <int DP, bool HALF, int SRC>
 __global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(Many<DP>::Occ, Many<DP>::Occ))) void
 paged_many_kernel(PagedAttnArgs a) {
     using S = Many<DP>;
-    __shared__ ManyLds<DP> lds;
+    extern __shared__ __align__(16) uint8_t many_lds[];
+    ManyLds<DP> &lds = *reinterpret_cast<ManyLds<DP> *>(many_lds);
     const int tid = int(threadIdx.x), lane = lane_id(), wave = tid >> 6, c = lane & 31, h = lane >> 5;
     int split, head, tile, seq;
     find_work(a, split, head, tile, seq);
@@ -736,20 +845,32 @@ paged_many_kernel(PagedAttnArgs a) {
     const uint16_t *kh = a.pool.k + int64_t(head) * a.pool.k_head;
     const uint16_t *vh = a.pool.v + int64_t(head) * a.pool.v_head;
     // channels past head_dim: K's are zero (they meet zero queries), V's feed outputs that nobody reads
-    for (int i = tid; i < S::KT * (DP - a.dim); i += kPagedThreads) {
-        const int t = i / (DP - a.dim), d = a.dim + i - t * (DP - a.dim);
-        lds.k[t * S::KR + d] = 0;
-        lds.v[t * S::VR + d] = 0;
+    for (int i = tid; i < 2 * S::KT * (DP - a.dim); i += kPagedThreads) {
+        const int t = i / (DP - a.dim), d = a.dim + i - t * (DP - a.dim), b = t / S::KT;
+        lds.buf[b].k[(t - b * S::KT) * S::KR + d] = 0;
+        lds.buf[b].v[(t - b * S::KT) * S::VR + d] = 0;
     }
+    // the queries, their sign turned where the scale is negative
+    const float scale2 = fabsf(a.scale2);
     u32x4a q[S::KS];
     {
+        const uint32_t flip = a.scale2 < 0.0f ? 0x80008000u : 0u;
         const int rr = min(row, r.count - 1);
         const uint16_t *qr = a.q.p + int64_t(row_token(a, r, rr)) * a.q.token +
                              int64_t(head * a.group + rr % a.group) * a.q.head;
 #pragma unroll
         for (int i = 0; i < S::KS; ++i) {
             const int ch = 16 * i + 8 * h;
-            q[i] = row < r.count && ch < a.dim ? *reinterpret_cast<const u32x4a *>(qr + ch) : u32x4a{0, 0, 0, 0};
+            q[i] = u32x4a{0, 0, 0, 0};
+            if (row < r.count && ch < a.dim) {
+                q[i] = *reinterpret_cast<const u32x4a *>(qr + ch);
+                if constexpr (SRC == 1) {
+                    const uint4 x = team::raw_octet(make_uint4(q[i][0], q[i][1], q[i][2], q[i][3]));
+                    q[i] = u32x4a{x.x, x.y, x.z, x.w};
+                }
+#pragma unroll
+                for (int n = 0; n < 4; ++n) q[i][n] ^= flip;
+            }
         }
     }
     f32x16 acc[S::CT];
@@ -759,153 +880,183 @@ paged_many_kernel(PagedAttnArgs a) {
         for (int i = 0; i < 16; ++i) acc[j][i] = 0.0f;
     float m = -__builtin_inff(), l = 0.0f;
 
-    // the next tile's rows on their way (pages)
-    u32x4a kn[S::NP], vn[S::NP];
-    auto find = [&](int tok) { // page and place of token tok + tid
-        int2 p = make_int2(0, 0);
-        if (tid < S::KT && tok < r.t1) p.x = page_at(a, table, min(tok + tid, r.t1 - 1), p.y);
-        return p;
-    };
-    auto request = [&](int tok) {
+    // ---- 32 tokens of a tile, from its half of LDS
+    auto work32 = [&](int tok, const uint16_t *kb, const uint16_t *vb, bool wild) {
+        f32x16 s;
 #pragma unroll
-        for (int k = 0; k < S::NP; ++k) {
-            const int o = tid + kPagedThreads * k, t = o / S::PR, ch = 8 * (o - t * S::PR);
-            const int2 at = lds.row[t];
-            kn[k] = vn[k] = u32x4a{0, 0, 0, 0};
-            if (ch < a.dim) {
-                kn[k] = *reinterpret_cast<const u32x4a *>(kh + int64_t(at.x) * a.pool.k_page +
-                                                          int64_t(at.y) * a.pool.k_token + ch);
-                if (tok + t < r.t1)
-                    vn[k] = *reinterpret_cast<const u32x4a *>(vh + int64_t(at.x) * a.pool.v_page +
-                                                              int64_t(at.y) * a.pool.v_token + ch);
-            }
+        for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::KS; ++i) {
+            const u32x4a kf = *reinterpret_cast<const u32x4a *>(kb + c * S::KR + 16 * i + 8 * h);
+            s = mfma32<HALF>(kf, q[i], s);
         }
-    };
-    if constexpr (SRC == 0) {
-        if (r.t0 < r.t1) {
-            const int2 p = find(r.t0);
-            if (tid < S::KT) lds.row[tid] = p;
-            __syncthreads();
-            request(r.t0);
+        // element i: token tok + 8 (i / 4) + 4 h + i % 4
+        if (tok + 32 > min(low, r.t1)) {
+            const int seen = min(limit, r.t1) - tok - 4 * h;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (8 * (i >> 2) + (i & 3) >= seen) s[i] = -__builtin_inff();
         }
-    }
-    for (int tok = r.t0; tok < r.t1; tok += S::KT) {
-        int2 next = make_int2(0, 0);
-        if constexpr (SRC == 0) next = find(tok + S::KT);
-        __syncthreads(); // the last tile is read
-        bool w = false;
-        const bool wg_cut = tok + S::KT > wg_low;
-        if constexpr (SRC == 0) {
+        float mt = s[0];
 #pragma unroll
-            for (int k = 0; k < S::NP; ++k) {
-                const int o = tid + kPagedThreads * k, t = o / S::PR, ch = 8 * (o - t * S::PR);
-                if (ch < a.dim) {
-                    *reinterpret_cast<u32x4a *>(lds.k + t * S::KR + ch) = kn[k];
-                    *reinterpret_cast<u32x4a *>(lds.v + t * S::VR + ch) = vn[k];
-                }
-                if (wg_cut)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w |= wild2<HALF>(vn[k][i]);
-            }
-            if (tid < S::KT) lds.row[tid] = next;
-        } else {
-            const PrefixTensor pk = a.px[2 * head], pv = a.px[2 * head + 1];
-            const int pt = tok / S::KT, rows = min(S::KT, r.len - tok);
-            stage_coded<S::KR, S::KT, false>(pk, pt, a.dim, rows, lds.k);
-            stage_coded<S::VR, S::KT, true>(pv, pt, a.dim, rows, lds.v);
-            __syncthreads();
-            patch_coded<S::KR>(pk, pt, a.dim, lds.k);
-            patch_coded<S::VR>(pv, pt, a.dim, lds.v);
-        }
-        bool wild = false;
-        if (SRC == 0 && wg_cut) wild = __syncthreads_or(w) != 0;
-        else __syncthreads();
-        if constexpr (SRC == 0)
-            if (tok + S::KT < r.t1) request(tok + S::KT);
-        if (!busy) continue;
-        f32x16 s[S::ST];
-#pragma unroll
-        for (int t = 0; t < S::ST; ++t) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < S::KS; ++i) {
-                const u32x4a kf = *reinterpret_cast<const u32x4a *>(lds.k + (32 * t + c) * S::KR + 16 * i + 8 * h);
-                s[t] = mfma32<HALF>(kf, q[i], s[t]);
-            }
-        }
-        // element i of tile t: token tok + 32 t + 8 (i / 4) + 4 h + i % 4
-        const int seen = min(limit, r.t1) - tok - 4 * h;
-        const bool cut = tok + S::KT > min(low, r.t1);
-        float mt = -__builtin_inff();
-#pragma unroll
-        for (int t = 0; t < S::ST; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[t][i] *= a.scale2;
-                if (cut && 32 * t + 8 * (i >> 2) + (i & 3) >= seen) s[t][i] = -__builtin_inff();
-                mt = fmaxf(mt, s[t][i]);
-            }
-        mt = fmaxf(mt, __shfl_xor(mt, 32));
+        for (int i = 1; i < 16; ++i) mt = fmaxf(mt, s[i]);
+        mt = fmaxf(mt, __shfl_xor(mt, 32)) * scale2;
         const float mn = fmaxf(m, mt);
         const float base = mn == -__builtin_inff() ? 0.0f : mn;
-        const float alpha = exp2_f32(m - base);
-        m = mn;
-        l *= alpha;
+        if (__ballot(mn != m) != 0) { // some row's maximum moves
+            const float alpha = exp2_f32(m - base);
+            l *= alpha;
 #pragma unroll
-        for (int t = 0; t < S::ST; ++t)
+            for (int j = 0; j < S::CT; ++j) acc[j] *= alpha;
+            m = mn;
+        }
+        float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[t][i] = exp2_f32(s[t][i] - base);
-                l += s[t][i];
-            }
-#pragma unroll
-        for (int j = 0; j < S::CT; ++j) acc[j] *= alpha;
-        // V: lane group lane / 16 reads channels 16 (group % 2) .. of tokens 4 (group / 2) ..
-        const uint16_t *vb = lds.v + ((lane & 15) >> 2) * S::VR + 4 * h * S::VR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        for (int i = 0; i < 16; ++i) {
+            s[i] = exp2_f32(__builtin_fmaf(s[i], scale2, -base));
+            sum += s[i];
+        }
+        l += sum;
         if (wild) {
             // An infinity or NaN among these tokens' V, and rows that do not
             // see all of them: a token at a time on the vector ALU, added only
             // where the row sees it, so that 0 times it stays out of the others.
 #pragma unroll 1
-            for (int u = 0; u < S::KT; ++u) {
+            for (int u = 0; u < 32; ++u) {
                 float pu = 0.0f;
 #pragma unroll
-                for (int t = 0; t < S::ST; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) pu = 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) == u ? s[t][i] : pu;
+                for (int i = 0; i < 16; ++i) pu = 8 * (i >> 2) + 4 * h + (i & 3) == u ? s[i] : pu;
                 pu += __shfl_xor(pu, 32); // (the other half of the lanes does not hold it)
                 if (tok + u >= limit || tok + u >= r.t1) continue;
-                const uint16_t *vu = lds.v + u * S::VR + 4 * h;
+                const uint16_t *vu = vb + u * S::VR + 4 * h;
 #pragma unroll
                 for (int j = 0; j < S::CT; ++j)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         acc[j][i] = __builtin_fmaf(pu, low_f32<HALF>(vu[32 * j + 8 * (i >> 2) + (i & 3)]), acc[j][i]);
             }
-            continue;
+            return;
         }
+        // V: lane group lane / 16 reads channels 16 (group % 2) .. of tokens 4 (group / 2) ..
+        const uint16_t *vl = vb + ((lane & 15) >> 2) * S::VR + 4 * h * S::VR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
-        for (int t = 0; t < S::ST; ++t)
+        for (int k = 0; k < 2; ++k) { // 16 tokens
+            u32x4a p;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) { // 16 tokens
-                u32x4a p;
+            for (int n = 0; n < 4; ++n) p[n] = pack2<HALF>(s[8 * k + 2 * n], s[8 * k + 2 * n + 1]);
 #pragma unroll
-                for (int n = 0; n < 4; ++n) p[n] = pack2<HALF>(s[t][8 * k + 2 * n], s[t][8 * k + 2 * n + 1]);
-#pragma unroll
-                for (int j = 0; j < S::CT; ++j) {
-                    const uint16_t *at = vb + (32 * t + 16 * k) * S::VR + 32 * j;
-                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at));
-                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 8 * S::VR));
-                    const uint2 x = __builtin_bit_cast(uint2, v0), y = __builtin_bit_cast(uint2, v1);
-                    acc[j] = mfma32<HALF>(u32x4a{x.x, x.y, y.x, y.y}, p, acc[j]);
-                }
+            for (int j = 0; j < S::CT; ++j) {
+                const uint16_t *at = vl + 16 * k * S::VR + 32 * j;
+                const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at));
+                const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 8 * S::VR));
+                const uint2 x = __builtin_bit_cast(uint2, v0), y = __builtin_bit_cast(uint2, v1);
+                acc[j] = mfma32<HALF>(u32x4a{x.x, x.y, y.x, y.y}, p, acc[j]);
             }
+        }
+    };
+    auto work = [&](int tok, const ManyBuf<DP> &buf, bool wild) {
+#pragma unroll XUNR
+        for (int t = 0; t < S::ST; ++t)
+            if (t == 0 || tok + 32 * t < r.t1) work32(tok + 32 * t, buf.k + 32 * t * S::KR, buf.v + 32 * t * S::VR, wild);
+    };
+
+    if (r.t0 < r.t1) {
+        if constexpr (SRC == 0) {
+            u32x4a kn[S::NP], vn[S::NP]; // the rows of a tile on their way
+            bool bad = false;
+            int2 place; // of one token of the tile after it
+            auto find = [&](int tok) {
+                const int t = min(tok + min(tid, S::KT - 1), r.t1 - 1);
+                const int col = page_of(a.pool, t);
+                place.x = table[col];
+                place.y = t - col * a.pool.page_tokens;
+            };
+            auto publish = [&](int slot) {
+                if (tid < S::KT) lds.row[slot][tid] = make_int2(held_page(a.pool, place.x, bad), place.y);
+            };
+            auto request = [&](int slot, int tok) {
+#pragma unroll
+                for (int k = 0; k < S::NP; ++k) {
+                    const int o = tid + kPagedThreads * k, t = o / S::PR, ch = min(8 * (o - t * S::PR), a.dim - 8);
+                    const int2 at = lds.row[slot][t];
+                    kn[k] = *reinterpret_cast<const u32x4a *>(
+                        kh + (int64_t(at.x) * a.pool.k_page + int64_t(at.y) * a.pool.k_token + ch));
+                    vn[k] = *reinterpret_cast<const u32x4a *>(
+                        vh + (int64_t(at.x) * a.pool.v_page + int64_t(at.y) * a.pool.v_token + ch));
+                }
+            };
+            // Tokens past the split's end: V is zero. Returns whether the tile
+            // holds an infinity or NaN in V where rows see different tokens of it.
+            auto store = [&](ManyBuf<DP> &buf, int tok) {
+                bool w = false;
+                const bool cut = tok + S::KT > wg_low;
+#pragma unroll
+                for (int k = 0; k < S::NP; ++k) {
+                    const int o = tid + kPagedThreads * k, t = o / S::PR, ch = 8 * (o - t * S::PR);
+                    u32x4a v = vn[k];
+                    if (tok + S::KT > r.t1 && tok + t >= r.t1) v = u32x4a{0, 0, 0, 0};
+                    if (cut)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w |= wild2<HALF>(v[i]);
+                    if (ch < a.dim) {
+                        *reinterpret_cast<u32x4a *>(buf.k + t * S::KR + ch) = kn[k];
+                        *reinterpret_cast<u32x4a *>(buf.v + t * S::VR + ch) = v;
+                    }
+                }
+                return cut && w;
+            };
+            int tok = r.t0;
+            find(tok);
+            publish(0);
+            find(tok + S::KT);
+            publish(1);
+            find(tok + 2 * S::KT);
+            __syncthreads();
+            request(0, tok);
+            bool w = store(lds.buf[0], tok);
+            request(1, tok + S::KT);
+            bool wild = __syncthreads_or(w) != 0;
+            for (int b = 0;; b ^= 1) {
+                if (busy) work(tok, lds.buf[b], wild);
+                if (tok + S::KT >= r.t1) break;
+                w = store(lds.buf[b ^ 1], tok + S::KT);
+                publish(b); // the tile after next; its rows are requested after the barrier
+                find(tok + 3 * S::KT);
+                wild = __syncthreads_or(w) != 0;
+                tok += S::KT;
+                if (tok + S::KT < r.t1) request(b, tok + S::KT);
+            }
+            if (bad) atomicOr(a.status, kStPage);
+        } else {
+            const PrefixSeg *ks = a.px[2 * head].segs, *vs = a.px[2 * head + 1].segs;
+            const int pr = a.dim / 8, last = (r.len - 1) / S::KT;
+            const Column at{8 * (tid % pr), tid / pr, kPagedThreads / pr};
+            CodedTile<DP> kt, vt;
+            PrefixSeg k0, v0; // the tile's first runs
+            auto request = [&](int t) {
+                k0 = ks[min(t, last)];
+                v0 = vs[min(t, last)];
+                coded_load<DP>(k0, a.dim, at, kt);
+                coded_load<DP>(v0, a.dim, at, vt);
+            };
+            int t = r.t0 / S::KT;
+            request(t);
+            for (int tok = r.t0, b = 0; tok < r.t1; tok += S::KT, ++t, b ^= 1) {
+                coded_store<DP, S::KR, false>(k0, ks, a.dim, at, kt, lds.buf[b].k);
+                coded_store<DP, S::VR, true>(v0, vs, a.dim, at, vt, lds.buf[b].v);
+                __syncthreads();
+                coded_patch<DP, S::KR>(k0, ks, a.dim, kt, lds.buf[b].k);
+                coded_patch<DP, S::VR>(v0, vs, a.dim, vt, lds.buf[b].v);
+                if (tok + S::KT < r.t1) request(t + 1);
+                __syncthreads();
+                if (busy) work(tok, lds.buf[b], false);
+            }
+        }
     }
     if (!busy) return;
     l += __shfl_xor(l, 32);
     if (row >= r.count) return;
-    // lane (c, h): row c, channels 32 j + 8 i + 4 h .. + 3
+    // lane (c, h): row c, places 32 j + 8 i + 4 h .. + 3 of the channels
     const int64_t slot = state_slot(a, r, head, split, row);
     const int64_t tok = row_token(a, r, row);
     const int hq = head * a.group + row % a.group;
@@ -923,14 +1074,18 @@ paged_many_kernel(PagedAttnArgs a) {
         for (int i = 0; i < 4; ++i) {
             const int ch = 32 * j + 8 * i + 4 * h;
             if (ch >= a.dim) continue;
-            if (a.direct) {
+            const float x0 = acc[j][4 * i], x1 = acc[j][4 * i + 1], x2 = acc[j][4 * i + 2], x3 = acc[j][4 * i + 3];
+            if constexpr (SRC == 1) { // octet order: channels 2 h, 2 h + 4, 2 h + 1, 2 h + 5 (never direct)
+                float *o = a.acc + slot * a.dim + (32 * j + 8 * i + 2 * h);
+                *reinterpret_cast<float2 *>(o) = make_float2(x0, x2);
+                *reinterpret_cast<float2 *>(o + 4) = make_float2(x1, x3);
+            } else if (a.direct) {
                 uint2 w;
-                w.x = pack2<HALF>(finish(acc[j][4 * i], l), finish(acc[j][4 * i + 1], l));
-                w.y = pack2<HALF>(finish(acc[j][4 * i + 2], l), finish(acc[j][4 * i + 3], l));
+                w.x = pack2<HALF>(finish(x0, l), finish(x1, l));
+                w.y = pack2<HALF>(finish(x2, l), finish(x3, l));
                 *reinterpret_cast<uint2 *>(a.out.p + tok * a.out.token + int64_t(hq) * a.out.head + ch) = w;
             } else {
-                *reinterpret_cast<float4 *>(a.acc + slot * a.dim + ch) =
-                    make_float4(acc[j][4 * i], acc[j][4 * i + 1], acc[j][4 * i + 2], acc[j][4 * i + 3]);
+                *reinterpret_cast<float4 *>(a.acc + slot * a.dim + ch) = make_float4(x0, x1, x2, x3);
             }
         }
 }

@@ -27,13 +27,22 @@ void launch_few(const PagedAttnArgs &a, bool two, int n_seqs, hipStream_t s) {
     halves ? launch_few_c<DP, HALF, 1, true>(a, n_seqs, s) : launch_few_c<DP, HALF, 1, false>(a, n_seqs, s);
 }
 
+template <int DP, bool HALF, int SRC>
+hipError_t launch_many_src(const PagedAttnArgs &a, int n_seqs, hipStream_t s) {
+    // (past the default 64 KiB of LDS at some sizes; set once per instantiation)
+    static const hipError_t set =
+        hipFuncSetAttribute(reinterpret_cast<const void *>(paged_many_kernel<DP, HALF, SRC>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(ManyLds<DP>)));
+    if (set != hipSuccess) return set;
+    hipLaunchKernelGGL((paged_many_kernel<DP, HALF, SRC>), attention_grid(a, n_seqs), dim3(kPagedThreads),
+                       sizeof(ManyLds<DP>), s, a);
+    return hipGetLastError();
+}
+
 template <int DP>
-void launch_many(const PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s) {
-    const dim3 grid = attention_grid(a, n_seqs);
-    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kPagedThreads), 0, s, a); };
-    if (a.px != nullptr) run(paged_many_kernel<DP, false, 1>);
-    else if (half) run(paged_many_kernel<DP, true, 0>);
-    else run(paged_many_kernel<DP, false, 0>);
+hipError_t launch_many(const PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s) {
+    if (a.px != nullptr) return launch_many_src<DP, false, 1>(a, n_seqs, s);
+    return half ? launch_many_src<DP, true, 0>(a, n_seqs, s) : launch_many_src<DP, false, 0>(a, n_seqs, s);
 }
 
 } // namespace paged
@@ -46,6 +55,5 @@ void launch_many(const PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s) {
         return hipGetLastError();                                                                                     \
     }                                                                                                                 \
     hipError_t paged_many_d##DP(const kvexp_dev::PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s) {            \
-        kvexp_dev::paged::launch_many<DP>(a, half, n_seqs, s);                                                        \
-        return hipGetLastError();                                                                                     \
+        return kvexp_dev::paged::launch_many<DP>(a, half, n_seqs, s);                                                 \
     }

@@ -74,7 +74,7 @@ struct RotateArgs {
 };
 
 // A run of rows of one block of a container that lie in one tile of the
-// shared prefix (kTileTokens).
+// shared prefix (tile_tokens).
 struct PrefixSeg {
     const uint8_t *data; // the block past its header
     const uint32_t *esc; // escape records of these rows
@@ -84,12 +84,13 @@ struct PrefixSeg {
     int32_t row0;        // first row, in the block
     int32_t rows;
     int32_t dst;         // first row in the tile
+    int32_t more, n_more; // further runs of the tile (blocks that end inside it): first and count
 };
 
-// One tensor (K or V of one head) of a shared prefix kept as containers.
+// One tensor (K or V of one head) of a shared prefix kept as containers: the
+// first run of every tile, then the further ones.
 struct PrefixTensor {
     const PrefixSeg *segs;
-    const int32_t *tile_seg; // first segment of each tile, n_tiles + 1 entries
 };
 
 // The attention calls. Partial states: slot (row, split) holds m, l (in the

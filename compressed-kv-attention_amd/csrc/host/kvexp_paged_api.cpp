@@ -309,10 +309,9 @@ void build_prefix(kvexp_hip_prefix &p, const kvexp_hip_head *heads, hipStream_t 
         std::copy(host + 1, host + 1 + total, e0.begin());
         std::copy(host + 1 + total, host + 1 + 2 * total, first.begin());
     }
-    // segments
+    // the runs of every tensor: each tile's first one, then the further ones
     const int tiles = (p.seq + kt - 1) / kt;
-    std::vector<PrefixSeg> segs;
-    std::vector<int32_t> tile_seg;
+    std::vector<PrefixSeg> segs, more;
     std::vector<size_t> seg_at, pos_at;
     std::vector<int2> blocks;
     size_t pos_total = 0;
@@ -324,12 +323,12 @@ void build_prefix(kvexp_hip_prefix &p, const kvexp_hip_head *heads, hipStream_t 
                 fail(KVEXP_HIP_FORMAT_ERROR, "xkv block index does not match the container");
         if (f[nb] < p.seq) fail(KVEXP_HIP_FORMAT_ERROR, "xkv ran out of tokens");
         seg_at.push_back(segs.size());
-        const size_t base = segs.size();
+        more.clear();
         int b = 0, tok = 0;
         for (int t = 0; t < tiles; ++t) {
-            tile_seg.push_back(int32_t(segs.size() - base));
             const int end = std::min(p.seq, (t + 1) * kt);
-            while (tok < end) {
+            const size_t head = segs.size();
+            for (bool is_first = true; tok < end; is_first = false) {
                 while (f[b + 1] <= tok) ++b;
                 PrefixSeg g{};
                 g.n_esc = i; // (see prefix_segs_kernel)
@@ -337,11 +336,17 @@ void build_prefix(kvexp_hip_prefix &p, const kvexp_hip_head *heads, hipStream_t 
                 g.row0 = tok - f[b];
                 g.rows = std::min(end, int(f[b + 1])) - tok;
                 g.dst = tok - t * kt;
-                segs.push_back(g);
                 tok += g.rows;
+                if (is_first) {
+                    g.more = int32_t(size_t(tiles) + more.size());
+                    segs.push_back(g);
+                } else {
+                    more.push_back(g);
+                    ++segs[head].n_more;
+                }
             }
         }
-        tile_seg.push_back(int32_t(segs.size() - base));
+        segs.insert(segs.end(), more.begin(), more.end());
         for (b = 0; b < nb; ++b) blocks.push_back(make_int2(i, b));
         pos_at.push_back(pos_total);
         pos_total += size_t(e0[at[size_t(i)] + size_t(nb)]);
@@ -351,8 +356,7 @@ void build_prefix(kvexp_hip_prefix &p, const kvexp_hip_head *heads, hipStream_t 
     // one allocation: what the host uploads, then the escape records
     const size_t o_tensors = padded(sizeof(uint32_t)), o_jobs = o_tensors + padded(size_t(n) * sizeof(PrefixTensor)),
                  o_blocks = o_jobs + padded(jobs_b), o_e0 = o_blocks + padded(blocks.size() * sizeof(int2)),
-                 o_tiles = o_e0 + padded(total * sizeof(int32_t)),
-                 o_segs = o_tiles + padded(tile_seg.size() * sizeof(int32_t)),
+                 o_segs = o_e0 + padded(total * sizeof(int32_t)),
                  o_pos = o_segs + padded(segs.size() * sizeof(PrefixSeg));
     const size_t pos_b = std::max<size_t>(1, pos_total) * sizeof(uint32_t);
     p.arena = DevBuf(o_pos + pos_b);
@@ -364,13 +368,11 @@ void build_prefix(kvexp_hip_prefix &p, const kvexp_hip_head *heads, hipStream_t 
         j.esc0 = reinterpret_cast<int32_t *>(d + o_e0) + at[size_t(i)];
         j.pos = reinterpret_cast<uint32_t *>(d + o_pos) + pos_at[size_t(i)];
         tensors[size_t(i)].segs = reinterpret_cast<const PrefixSeg *>(d + o_segs) + seg_at[size_t(i)];
-        tensors[size_t(i)].tile_seg = reinterpret_cast<const int32_t *>(d + o_tiles) + size_t(i) * size_t(tiles + 1);
     }
     std::memcpy(image.data() + o_tensors, tensors.data(), tensors.size() * sizeof(PrefixTensor));
     std::memcpy(image.data() + o_jobs, jobs.data(), jobs_b);
     std::memcpy(image.data() + o_blocks, blocks.data(), blocks.size() * sizeof(int2));
     std::memcpy(image.data() + o_e0, e0.data(), total * sizeof(int32_t));
-    std::memcpy(image.data() + o_tiles, tile_seg.data(), tile_seg.size() * sizeof(int32_t));
     std::memcpy(image.data() + o_segs, segs.data(), segs.size() * sizeof(PrefixSeg));
     SyncOnExit sync{s};
     HIPX(hipMemcpyAsync(d, image.data(), image.size(), hipMemcpyHostToDevice, s));
