@@ -669,7 +669,7 @@ struct alignas(16) ManyBuf {
 template <int DP>
 struct alignas(16) ManyLds {
     ManyBuf<DP> buf[2];
-    int2 row[2][Many<DP>::KT]; // page and place of the tokens of tiles on their way
+    longlong2 row[2][Many<DP>::KT]; // where K and V of the tokens of tiles on their way begin
 };
 
 typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
@@ -685,23 +685,44 @@ __device__ __forceinline__ int octet_place(int ch) { return (ch & ~7) | ((ch & 3
 // 8 channels of one row of a run, as they lie in the container.
 struct CodedOctet {
     uint2 sm; // sign/mantissa bytes (a plain block: the first 8 bytes)
-    uint2 c;  // x: the codes (a plain block: the other 8 bytes)
+    uint2 c;  // x: the codes, at its upper end (a plain block: the other 8 bytes)
 };
 
-// The octet from channel ch of row `row` of a run.
-__device__ __forceinline__ void load_octet(const PrefixSeg &s, int dim, int row, int ch, CodedOctet &o) {
-    const int e = (s.row0 + row) * dim + ch; // element of the block
-    const uint8_t *p = s.mode == 0 ? s.data + 2 * e : s.data + dim + e;
-    const any_u32x2 sm = *reinterpret_cast<const any_u32x2 *>(p);
-    o.sm = make_uint2(sm.x, sm.y);
-    const uint8_t *cp = s.data + dim + s.n_tokens * dim + (e >> 3) * s.mode;
-    if (s.mode == 4) o.c.x = *reinterpret_cast<const any_u32 *>(cp);
-    else if (s.mode == 2) o.c.x = *reinterpret_cast<const any_u16 *>(cp);
-    else if (s.mode == 3) o.c.x = uint32_t(*reinterpret_cast<const any_u16 *>(cp)) | (uint32_t(cp[2]) << 16);
-    else {
-        const any_u32x2 x = *reinterpret_cast<const any_u32x2 *>(p + 8);
-        o.c = make_uint2(x.x, x.y);
+// A run, read through the scalar cache (the same in every lane; the tables do
+// not change while a prefix lives).
+typedef const __attribute__((address_space(4))) PrefixSeg c_seg;
+__device__ __forceinline__ PrefixSeg seg_at(const PrefixSeg *segs, int i) {
+    c_seg *p = (c_seg *)(uintptr_t)(segs + i);
+    PrefixSeg s;
+    s.data = p->data;
+    s.esc = p->esc;
+    s.n_esc = p->n_esc;
+    s.mode = p->mode;
+    s.n_tokens = p->n_tokens;
+    s.row0 = p->row0;
+    s.rows = p->rows;
+    s.dst = p->dst;
+    s.more = p->more;
+    s.n_more = p->n_more;
+    return s;
+}
+
+// The octet from channel ch of row `row` of a run; `plain`: its mode is 0. The
+// codes come as the dword that ends with them (bytes of the block before them
+// in front), so that no load reaches past the block.
+__device__ __forceinline__ void load_octet(const PrefixSeg &s, bool plain, int dim, int row, int ch, CodedOctet &o) {
+    const uint32_t e = uint32_t((s.row0 + row) * dim + ch); // element of the block
+    if (plain) {
+        const any_u32x2 a = *reinterpret_cast<const any_u32x2 *>(s.data + 2 * e),
+                        b = *reinterpret_cast<const any_u32x2 *>(s.data + (2 * e + 8));
+        o.sm = make_uint2(a.x, a.y);
+        o.c = make_uint2(b.x, b.y);
+        return;
     }
+    const any_u32x2 sm = *reinterpret_cast<const any_u32x2 *>(s.data + (uint32_t(dim) + e));
+    o.sm = make_uint2(sm.x, sm.y);
+    const uint8_t *codes = s.data + (dim + s.n_tokens * dim + s.mode - 4);
+    o.c = make_uint2(*reinterpret_cast<const any_u32 *>(codes + (e >> 3) * uint32_t(s.mode)), 0);
 }
 
 // The octet's BF16 words in octet order (escapes come after), from its base
@@ -710,8 +731,8 @@ template <int MODE>
 __device__ __forceinline__ u32x4a decode_octet(const CodedOctet &o, const uint32_t (&bp)[4], uint32_t smm) {
     uint32_t cw, t[4];
     if constexpr (MODE == 4) cw = o.c.x;
-    else if constexpr (MODE == 2) cw = __builtin_amdgcn_perm(o.c.x, o.c.x, 0x0c010c00u);
-    else cw = (o.c.x & 0xFFFu) | ((o.c.x << 4) & 0x0FFF0000u);
+    else if constexpr (MODE == 2) cw = __builtin_amdgcn_perm(o.c.x, o.c.x, 0x0c030c02u);
+    else cw = ((o.c.x >> 8) & 0xFFFu) | ((o.c.x >> 4) & 0x0FFF0000u);
     team::octet_exponents<MODE>(cw, bp, t);
     return u32x4a{team::team_pair(o.sm.x, o.sm.y, 0, t[0], smm), team::team_pair(o.sm.x, o.sm.y, 1, t[1], smm),
                   team::team_pair(o.sm.x, o.sm.y, 2, t[2], smm), team::team_pair(o.sm.x, o.sm.y, 3, t[3], smm)};
@@ -746,12 +767,18 @@ __device__ __forceinline__ void coded_load(const PrefixSeg &s, int dim, const Co
     const int tid = int(threadIdx.x);
     t.rec = s.esc[max(min(tid, s.n_esc - 1), 0)];
     const int lastp = s.rows - 1;
+    // (a plain block has no base exponents; it starts with at least a row)
+    const any_u32x2 b = *reinterpret_cast<const any_u32x2 *>(s.data + at.ch);
+    t.base = make_uint2(b.x, b.y);
     if (s.mode != 0) {
-        const any_u32x2 b = *reinterpret_cast<const any_u32x2 *>(s.data + at.ch);
-        t.base = make_uint2(b.x, b.y);
-    }
 #pragma unroll
-    for (int k = 0; k < Many<DP>::NR; ++k) load_octet(s, dim, min(at.row + at.step * k, lastp), at.ch, t.o[k]);
+        for (int k = 0; k < Many<DP>::NR; ++k)
+            load_octet(s, false, dim, min(at.row + at.step * k, lastp), at.ch, t.o[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < Many<DP>::NR; ++k)
+            load_octet(s, true, dim, min(at.row + at.step * k, lastp), at.ch, t.o[k]);
+    }
 }
 
 // The run's rows to LDS rows of R elements; V: the tile's other rows are zero
@@ -782,7 +809,7 @@ __device__ __forceinline__ void coded_store(const PrefixSeg &s, const PrefixSeg 
     // blocks that end inside the tile: their rows are read here
     int end = s.rows;
     for (int i = 0; i < s.n_more; ++i) {
-        const PrefixSeg g = segs[s.more + i];
+        const PrefixSeg g = seg_at(segs, s.more + i);
         end = g.dst + g.rows;
         uint2 base = make_uint2(0, 0);
         if (g.mode != 0) {
@@ -792,7 +819,7 @@ __device__ __forceinline__ void coded_store(const PrefixSeg &s, const PrefixSeg 
         base_words(base, bp);
         for (int row = at.row; mine && row < g.rows; row += at.step) {
             CodedOctet o;
-            load_octet(g, dim, row, at.ch, o);
+            load_octet(g, g.mode == 0, dim, row, at.ch, o);
             *reinterpret_cast<u32x4a *>(lds + (g.dst + row) * R + at.ch) =
                 g.mode == 4   ? decode_octet<4>(o, bp, smm)
                 : g.mode == 2 ? decode_octet<2>(o, bp, smm)
@@ -819,7 +846,7 @@ __device__ __forceinline__ void coded_patch(const PrefixSeg &s, const PrefixSeg 
     if (tid < s.n_esc) patch_one<R>(s, dim, t.rec, lds);
     for (int i = tid + kPagedThreads; i < s.n_esc; i += kPagedThreads) patch_one<R>(s, dim, s.esc[i], lds);
     for (int k = 0; k < s.n_more; ++k) {
-        const PrefixSeg g = segs[s.more + k];
+        const PrefixSeg g = seg_at(segs, s.more + k);
         for (int i = tid; i < g.n_esc; i += kPagedThreads) patch_one<R>(g, dim, g.esc[i], lds);
     }
 }
@@ -859,18 +886,16 @@ paged_many_kernel(PagedAttnArgs a) {
         const uint16_t *qr = a.q.p + int64_t(row_token(a, r, rr)) * a.q.token +
                              int64_t(head * a.group + rr % a.group) * a.q.head;
 #pragma unroll
-        for (int i = 0; i < S::KS; ++i) {
-            const int ch = 16 * i + 8 * h;
-            q[i] = u32x4a{0, 0, 0, 0};
-            if (row < r.count && ch < a.dim) {
-                q[i] = *reinterpret_cast<const u32x4a *>(qr + ch);
-                if constexpr (SRC == 1) {
-                    const uint4 x = team::raw_octet(make_uint4(q[i][0], q[i][1], q[i][2], q[i][3]));
-                    q[i] = u32x4a{x.x, x.y, x.z, x.w};
-                }
+        for (int i = 0; i < S::KS; ++i) q[i] = *reinterpret_cast<const u32x4a *>(qr + min(16 * i + 8 * h, a.dim - 8));
 #pragma unroll
-                for (int n = 0; n < 4; ++n) q[i][n] ^= flip;
+        for (int i = 0; i < S::KS; ++i) {
+            if constexpr (SRC == 1) {
+                const uint4 x = team::raw_octet(make_uint4(q[i][0], q[i][1], q[i][2], q[i][3]));
+                q[i] = u32x4a{x.x, x.y, x.z, x.w};
             }
+            const bool none = row >= r.count || 16 * i + 8 * h >= a.dim;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) q[i][n] = none ? 0u : q[i][n] ^ flip;
         }
     }
     f32x16 acc[S::CT];
@@ -890,6 +915,17 @@ paged_many_kernel(PagedAttnArgs a) {
             const u32x4a kf = *reinterpret_cast<const u32x4a *>(kb + c * S::KR + 16 * i + 8 * h);
             s = mfma32<HALF>(kf, q[i], s);
         }
+#ifndef XNOSCHED
+        // a few rows of K ahead of the products (else each product waits for its own)
+        constexpr int Deep = S::KS < 4 ? S::KS : 4;
+        __builtin_amdgcn_sched_group_barrier(0x100, Deep, 0);
+#pragma unroll
+        for (int i = 0; i < S::KS - Deep; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, Deep, 0);
+#endif
         // element i: token tok + 8 (i / 4) + 4 h + i % 4
         if (tok + 32 > min(low, r.t1)) {
             const int seen = min(limit, r.t1) - tok - 4 * h;
@@ -972,17 +1008,18 @@ paged_many_kernel(PagedAttnArgs a) {
                 place.y = t - col * a.pool.page_tokens;
             };
             auto publish = [&](int slot) {
-                if (tid < S::KT) lds.row[slot][tid] = make_int2(held_page(a.pool, place.x, bad), place.y);
+                if (tid >= S::KT) return;
+                const int64_t page = held_page(a.pool, place.x, bad);
+                lds.row[slot][tid] = make_longlong2(page * a.pool.k_page + int64_t(place.y) * a.pool.k_token,
+                                                    page * a.pool.v_page + int64_t(place.y) * a.pool.v_token);
             };
             auto request = [&](int slot, int tok) {
 #pragma unroll
                 for (int k = 0; k < S::NP; ++k) {
                     const int o = tid + kPagedThreads * k, t = o / S::PR, ch = min(8 * (o - t * S::PR), a.dim - 8);
-                    const int2 at = lds.row[slot][t];
-                    kn[k] = *reinterpret_cast<const u32x4a *>(
-                        kh + (int64_t(at.x) * a.pool.k_page + int64_t(at.y) * a.pool.k_token + ch));
-                    vn[k] = *reinterpret_cast<const u32x4a *>(
-                        vh + (int64_t(at.x) * a.pool.v_page + int64_t(at.y) * a.pool.v_token + ch));
+                    const longlong2 at = lds.row[slot][t];
+                    kn[k] = *reinterpret_cast<const u32x4a *>(kh + (at.x + ch));
+                    vn[k] = *reinterpret_cast<const u32x4a *>(vh + (at.y + ch));
                 }
             };
             // Tokens past the split's end: V is zero. Returns whether the tile
@@ -1034,8 +1071,8 @@ paged_many_kernel(PagedAttnArgs a) {
             CodedTile<DP> kt, vt;
             PrefixSeg k0, v0; // the tile's first runs
             auto request = [&](int t) {
-                k0 = ks[min(t, last)];
-                v0 = vs[min(t, last)];
+                k0 = seg_at(ks, min(t, last));
+                v0 = seg_at(vs, min(t, last));
                 coded_load<DP>(k0, a.dim, at, kt);
                 coded_load<DP>(v0, a.dim, at, vt);
             };
