@@ -19,6 +19,8 @@
 #include "attention_team.h"
 #include "paged_device.h"
 
+#include <type_traits>
+
 #include <hip/hip_fp16.h>
 
 namespace kvexp_dev {
@@ -85,6 +87,31 @@ __device__ __forceinline__ bool wild2(uint32_t w) {
     constexpr uint32_t E = HALF ? 0x7C00u : 0x7F80u;
     return (w & E) == E || (w & (E << 16)) == (E << 16);
 }
+
+// Infinities and NaN among V of tokens that some rows of a tile see and others
+// do not: the product with P would carry 0 times them into the rows that do not.
+// Such a tile takes its product without them, and a second one, of 1 in their
+// places and 1 for the tokens that a row sees, says which outputs they reach:
+// those get an infinity of their sign, or NaN (both signs).
+template <bool HALF>
+struct Wild {
+    static constexpr uint32_t E = HALF ? 0x7C00u : 0x7F80u, One = HALF ? 0x3C00u : 0x3F80u;
+    // the halves that are finite, the others 0
+    static __device__ __forceinline__ uint32_t without(uint32_t w) {
+        const uint32_t lo = (w & E) == E ? 0xFFFFu : 0u, hi = (w & (E << 16)) == (E << 16) ? 0xFFFF0000u : 0u;
+        return w & ~(lo | hi);
+    }
+    // 1 where a half reaches plus (or minus) infinity or NaN
+    static __device__ __forceinline__ uint32_t only(uint32_t w, bool minus) {
+        auto half = [&](uint32_t x) { // plus: all but -inf; minus: all but +inf
+            return (x & E) == E && x != (minus ? E : (E | 0x8000u)) ? One : 0u;
+        };
+        return half(w & 0xFFFFu) | (half(w >> 16) << 16);
+    }
+    static __device__ __forceinline__ float reach(float z, bool minus) {
+        return z > 0.0f ? (minus ? -__builtin_inff() : __builtin_inff()) : 0.0f;
+    }
+};
 
 // The rows of a workgroup: which query rows, which tokens they see.
 struct Rows {
@@ -228,8 +255,6 @@ struct Few {
     static constexpr int VW = C / 2;     // their dwords
     static constexpr int JC = DP > 192 ? DP / 2 : DP; // channels joined at a time (LDS below 64 KiB)
     static constexpr int Row = JC + 4;   // floats per row of the joint state
-    template <bool CAUSAL>
-    static constexpr int Lds = 16 * kPagedWaves * (CAUSAL && DP > Row ? 4 * DP : 4 * Row);
     // A second tile in registers, and the waves per SIMD that the registers then
     // allow. More waves hide more than a tile ahead does where both do not fit:
     // four sequences of up to 65,536 tokens, 8 heads x 4 queries of 128 channels,
@@ -244,9 +269,10 @@ struct Few {
     // channels: 87 -> 80 us; at 128 channels it spills, 118 -> 142).
     static constexpr bool Early = DP > 192;
     template <int NC, bool CAUSAL>
-    static constexpr int Occ = NC > 1 ? 2
+    static constexpr int Occ = CAUSAL ? (DP <= 96 || (DP == 128 && NC == 1) ? 2 : 1)
+                               : NC > 1 ? 2
                                : DP <= 32 ? 4
-                               : DP <= 128 ? (CAUSAL && DP % 64 == 0 ? 2 : 3)
+                               : DP <= 128 ? 3
                                : DP <= 192 ? 2 : 1;
 };
 
@@ -323,7 +349,7 @@ template <int DP, bool HALVES, bool V>
 __device__ __forceinline__ void few_load(const PagedAttnArgs &a, const uint16_t *base, int tok, int last, int vc,
                                          const FewPlaces<HALVES> &p, bool &bad, FewTile<DP> &f) {
     using F = Few<DP>;
-    const int lane = lane_id(), c = lane & 15, g = lane >> 4;
+    const int lane = wave::lane_here(), c = lane & 15, g = lane >> 4; // (not held across the loop)
     const int64_t page_step = V ? a.pool.v_page : a.pool.k_page, token_step = V ? a.pool.v_token : a.pool.k_token;
     auto key = [&](const uint16_t *row, int j) {
 #pragma unroll
@@ -374,9 +400,7 @@ template <int DP, bool HALF, int NC, bool HALVES, bool CAUSAL>
 __global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(Few<DP>::template Occ<NC, CAUSAL>, Few<DP>::template Occ<NC, CAUSAL>))) void
 paged_few_kernel(PagedAttnArgs a) {
     using F = Few<DP>;
-    // the waves' states at the end; before, a wave's V of a tile that needs care (below)
-    __shared__ __align__(16) uint8_t lds[F::template Lds<CAUSAL>];
-    float(*joint)[16][F::Row] = reinterpret_cast<float(*)[16][F::Row]>(lds);
+    __shared__ float joint[kPagedWaves][16][F::Row];
     const int lane = lane_id(), c = lane & 15, g = lane >> 4, wave = int(threadIdx.x) >> 6;
     int split, head, tile, seq;
     find_work(a, split, head, tile, seq);
@@ -418,7 +442,9 @@ paged_few_kernel(PagedAttnArgs a) {
     const int last = r.t1 - 1;
 
     // one tile; once K has given its scores, `keys_done` may request others in its place
-    auto work = [&](FewTile<DP> &f, int tok, auto keys_done) {
+    // (CUT: some row does not see some of these tokens)
+    auto work = [&](auto cut_tile, FewTile<DP> &f, int tok, auto keys_done) {
+        constexpr bool cut = decltype(cut_tile)::value;
         if (a.dim != DP) { // channels past head_dim: zero, as their queries are
 #pragma unroll
             for (int i = 0; i < F::KS; ++i)
@@ -426,9 +452,9 @@ paged_few_kernel(PagedAttnArgs a) {
                 for (int j = 0; j < 2; ++j)
                     if (32 * i + 8 * g >= a.dim) f.k[j][i] = u32x4a{0, 0, 0, 0};
         }
-        const bool cut = tok + 32 > min(low, r.t1); // some row does not see some of these tokens
         bool wild = false;
-        if (cut) {
+        const bool now = cut && tok + 32 > min(low, r.t1);
+        if (now) {
             if constexpr (CAUSAL) {
                 bool w = false;
 #pragma unroll
@@ -460,7 +486,7 @@ paged_few_kernel(PagedAttnArgs a) {
             float p[8];
 #pragma unroll
             for (int n = 0; n < 8; ++n) p[n] = s[x][n >> 2][n & 3] * a.scale2;
-            if (cut) {
+            if (now) {
                 const int seen = min(limit[x], r.t1) - (tok + 4 * g); // lane's token n is seen if off(n) < seen
 #pragma unroll
                 for (int n = 0; n < 8; ++n)
@@ -491,49 +517,45 @@ paged_few_kernel(PagedAttnArgs a) {
                 lo[x][n] = pack2<HALF>(p[2 * n] - low_f32<HALF>(hi[x][n]), p[2 * n + 1] - high_f32<HALF>(hi[x][n]));
             }
         }
-        if (!CAUSAL || !wild) {
+        using W = Wild<HALF>;
 #pragma unroll
-            for (int j = 0; j < F::C; ++j) {
-                const u32x4a v = few_v<DP>(f, j);
+        for (int j = 0; j < F::C; ++j) {
+            u32x4a v = few_v<DP>(f, j);
+            if constexpr (CAUSAL && cut) {
 #pragma unroll
-                for (int x = 0; x < NC; ++x) {
-                    acc[x][j] = mfma16<HALF>(v, hi[x], acc[x][j]);
-                    acc[x][j] = mfma16<HALF>(v, lo[x], acc[x][j]);
-                }
+                for (int n = 0; n < 4; ++n) v[n] = W::without(v[n]);
             }
-            return;
-        }
-        // An infinity or NaN among these tokens' V, and rows that do not see
-        // all of them: a token at a time on the vector ALU, added only where the
-        // row sees it, so that 0 times it stays out of the others.
-        uint32_t *vl = reinterpret_cast<uint32_t *>(lds) + wave * (16 * DP); // V of the tile, a row of DP per token
-#pragma unroll
-        for (int n = 0; n < 8; ++n)
-#pragma unroll
-            for (int k = 0; k < F::VW; ++k) vl[((4 * g + (n & 3) + 16 * (n >> 2)) * DP + vc) / 2 + k] = f.v[n][k];
-#pragma unroll 1
-        for (int u = 0; u < 32; ++u) { // place un of lane group ug
-            const int ug = (u >> 2) & 3, un = (u & 3) + 4 * (u >> 4);
 #pragma unroll
             for (int x = 0; x < NC; ++x) {
-                uint32_t h = 0, w = 0;
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    h = n == (un >> 1) ? hi[x][n] : h;
-                    w = n == (un >> 1) ? lo[x][n] : w;
-                }
-                const float mine = un & 1 ? high_f32<HALF>(h) + high_f32<HALF>(w) : low_f32<HALF>(h) + low_f32<HALF>(w);
-                const float pu = __shfl(mine, c + 16 * ug);
-                if (tok + u >= limit[x] || tok + u >= r.t1) continue;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int k = 0; k < F::VW; ++k) {
-                        const uint32_t v = vl[(u * DP + min(F::C * (4 * g + i), a.dim - F::C)) / 2 + k];
-                        acc[x][2 * k][i] = __builtin_fmaf(pu, low_f32<HALF>(v), acc[x][2 * k][i]);
-                        acc[x][2 * k + 1][i] = __builtin_fmaf(pu, high_f32<HALF>(v), acc[x][2 * k + 1][i]);
-                    }
+                acc[x][j] = mfma16<HALF>(v, hi[x], acc[x][j]);
+                acc[x][j] = mfma16<HALF>(v, lo[x], acc[x][j]);
             }
+        }
+        if constexpr (CAUSAL && cut) {
+            if (!wild) return;
+#pragma unroll
+            for (int j = 0; j < F::C; ++j)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    u32x4a v = few_v<DP>(f, j), sees;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) v[n] = W::only(v[n], s != 0);
+#pragma unroll
+                    for (int x = 0; x < NC; ++x) {
+                        const int seen = min(limit[x], r.t1) - (tok + 4 * g);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const int at = ((2 * n) & 3) + 16 * (n >> 1);
+                            sees[n] = (at < seen ? W::One : 0u) | (at + 1 < seen ? W::One << 16 : 0u);
+                        }
+                        f32x4 z = {0, 0, 0, 0};
+                        z = mfma16<HALF>(v, sees, z);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) z[i] = W::reach(z[i], s != 0);
+                        acc[x][j] += z;
+                        __builtin_amdgcn_sched_barrier(0); // (one at a time: registers)
+                    }
+                }
         }
     };
 
@@ -549,33 +571,40 @@ paged_few_kernel(PagedAttnArgs a) {
         keys(tok, f0);
         values(tok, f0);
         places(tok + Step);
+        using Whole = std::integral_constant<bool, false>;
+        using Cut = std::integral_constant<bool, true>;
+        const int whole = min(low, r.t1) - 32; // tiles up to here are seen whole by every row
         if constexpr (F::template Ahead<NC>) {
             FewTile<DP> f1;
-            for (;;) {
-                keys(tok + Step, f1);
-                values(tok + Step, f1);
+            auto next_tile = [&](FewTile<DP> &f) {
+                keys(tok + Step, f);
+                values(tok + Step, f);
                 places(tok + 2 * Step);
-                work(f0, tok, [] {});
+            };
+            auto turn = [&](FewTile<DP> &f, FewTile<DP> &g) {
+                next_tile(g);
+                if (CAUSAL && tok <= whole) work(Whole{}, f, tok, [] {});
+                else work(Cut{}, f, tok, [] {});
                 tok += Step;
-                if (tok >= r.t1) break;
-                keys(tok + Step, f0);
-                values(tok + Step, f0);
-                places(tok + 2 * Step);
-                work(f1, tok, [] {});
-                tok += Step;
-                if (tok >= r.t1) break;
-            }
+                return tok < r.t1;
+            };
+            while (turn(f0, f1) && turn(f1, f0)) {}
         } else {
-            for (;;) {
-                work(f0, tok, [&] {
+            auto turn = [&](auto cut) {
+                work(cut, f0, tok, [&] {
                     if constexpr (F::Early) keys(tok + Step, f0);
                 });
                 tok += Step;
-                if (tok >= r.t1) break;
+                if (tok >= r.t1) return false;
                 if constexpr (!F::Early) keys(tok, f0);
                 values(tok, f0);
                 places(tok + Step);
-            }
+                return true;
+            };
+            bool more = true;
+            if constexpr (CAUSAL)
+                while (more && tok <= whole) more = turn(Whole{});
+            while (more) more = turn(Cut{});
         }
         if (bad) atomicOr(a.status, kStPage);
     }
@@ -588,7 +617,7 @@ paged_few_kernel(PagedAttnArgs a) {
         l[x] += __shfl_xor(l[x], 16);
         l[x] += __shfl_xor(l[x], 32);
         for (int d0 = 0; d0 < a.dim; d0 += F::JC) {
-            __syncthreads(); // (the states before, or a wave's V, are read)
+            if (x > 0 || d0 > 0) __syncthreads();
             if (g == 0 && d0 == 0) {
                 joint[wave][c][F::JC] = m[x];
                 joint[wave][c][F::JC + 1] = l[x];
@@ -623,6 +652,14 @@ paged_few_kernel(PagedAttnArgs a) {
     }
 }
 
+// threadIdx.x as the compiler does not know it: what follows from it is computed
+// where it is used instead of being held in registers across a loop.
+__device__ __forceinline__ int thread_here() {
+    int t = int(threadIdx.x);
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
 // -------------------------------------------------------------- many rows --
 // Up to 128 query rows per workgroup, 32 per wave (32 x 32 x 16 products):
 // prompts in chunks, draft tokens, and the rows of a whole batch against a
@@ -641,9 +678,6 @@ paged_few_kernel(PagedAttnArgs a) {
 // (containers: twice, the escapes being written over their elements between),
 // and two workgroups share a CU, so that one's products run beside the other's
 // exponentials.
-#ifndef XUNR
-#define XUNR 1
-#endif
 template <int DP>
 struct Many {
     static constexpr int KT = tile_tokens(DP);
@@ -669,7 +703,7 @@ struct alignas(16) ManyBuf {
 template <int DP>
 struct alignas(16) ManyLds {
     ManyBuf<DP> buf[2];
-    longlong2 row[2][Many<DP>::KT]; // where K and V of the tokens of tiles on their way begin
+    longlong2 row[2][Many<DP>::KT]; // where K and V of the tokens of tiles on their way begin (bytes)
 };
 
 typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
@@ -762,22 +796,41 @@ struct Column {
     int ch, row, step;
 };
 
+// Whether a run fills the tile and its rows the passes (the usual case): then a
+// pass is a fixed step of the streams after the one before.
+template <int DP>
+__device__ __forceinline__ bool whole_run(const PrefixSeg &s, int dim) {
+    return s.rows == Many<DP>::KT && dim == DP && kPagedThreads % Many<DP>::PR == 0;
+}
+
 template <int DP>
 __device__ __forceinline__ void coded_load(const PrefixSeg &s, int dim, const Column &at, CodedTile<DP> &t) {
-    const int tid = int(threadIdx.x);
+    using S = Many<DP>;
+    const int tid = thread_here();
     t.rec = s.esc[max(min(tid, s.n_esc - 1), 0)];
-    const int lastp = s.rows - 1;
     // (a plain block has no base exponents; it starts with at least a row)
-    const any_u32x2 b = *reinterpret_cast<const any_u32x2 *>(s.data + at.ch);
+    const any_u32x2 b = *reinterpret_cast<const any_u32x2 *>(s.data + uint32_t(at.ch));
     t.base = make_uint2(b.x, b.y);
+    if (s.mode != 0 && whole_run<DP>(s, dim)) {
+        const uint32_t e0 = uint32_t(8 * tid); // element of the run
+        const uint8_t *sm = s.data + (DP + s.row0 * DP),
+                      *codes = s.data + (DP + s.n_tokens * DP + s.row0 * (DP / 8) * s.mode + s.mode - 4);
+        const uint32_t c0 = uint32_t(tid) * uint32_t(s.mode);
+#pragma unroll
+        for (int k = 0; k < S::NR; ++k) {
+            const any_u32x2 x = *reinterpret_cast<const any_u32x2 *>(sm + 8 * kPagedThreads * k + e0);
+            t.o[k].sm = make_uint2(x.x, x.y);
+            t.o[k].c = make_uint2(*reinterpret_cast<const any_u32 *>(codes + kPagedThreads * k * s.mode + c0), 0);
+        }
+        return;
+    }
+    const int lastp = s.rows - 1;
     if (s.mode != 0) {
 #pragma unroll
-        for (int k = 0; k < Many<DP>::NR; ++k)
-            load_octet(s, false, dim, min(at.row + at.step * k, lastp), at.ch, t.o[k]);
+        for (int k = 0; k < S::NR; ++k) load_octet(s, false, dim, min(at.row + at.step * k, lastp), at.ch, t.o[k]);
     } else {
 #pragma unroll
-        for (int k = 0; k < Many<DP>::NR; ++k)
-            load_octet(s, true, dim, min(at.row + at.step * k, lastp), at.ch, t.o[k]);
+        for (int k = 0; k < S::NR; ++k) load_octet(s, true, dim, min(at.row + at.step * k, lastp), at.ch, t.o[k]);
     }
 }
 
@@ -790,6 +843,12 @@ __device__ __forceinline__ void coded_store(const PrefixSeg &s, const PrefixSeg 
     const uint32_t smm = wave::sm_mask_vgpr();
     const bool mine = at.row < at.step; // (threads past the whole rows of a pass have none)
     auto put = [&](auto octet) {
+        if (whole_run<DP>(s, dim)) {
+            uint16_t *to = lds + at.row * R + at.ch;
+#pragma unroll
+            for (int k = 0; k < S::NR; ++k) *reinterpret_cast<u32x4a *>(to + k * S::RP * R) = octet(k);
+            return;
+        }
 #pragma unroll
         for (int k = 0; k < S::NR; ++k) {
             const int row = at.row + at.step * k;
@@ -906,7 +965,9 @@ paged_many_kernel(PagedAttnArgs a) {
     float m = -__builtin_inff(), l = 0.0f;
 
     // ---- 32 tokens of a tile, from its half of LDS
-    auto work32 = [&](int tok, const uint16_t *kb, const uint16_t *vb, bool wild) {
+    // (CUT: some row of the workgroup does not see all of the tile)
+    auto work32 = [&](auto cut, int tok, const uint16_t *kb, const uint16_t *vb, bool wild) {
+        constexpr bool CUT = decltype(cut)::value;
         f32x16 s;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = 0.0f;
@@ -915,7 +976,6 @@ paged_many_kernel(PagedAttnArgs a) {
             const u32x4a kf = *reinterpret_cast<const u32x4a *>(kb + c * S::KR + 16 * i + 8 * h);
             s = mfma32<HALF>(kf, q[i], s);
         }
-#ifndef XNOSCHED
         // a few rows of K ahead of the products (else each product waits for its own)
         constexpr int Deep = S::KS < 4 ? S::KS : 4;
         __builtin_amdgcn_sched_group_barrier(0x100, Deep, 0);
@@ -925,9 +985,8 @@ paged_many_kernel(PagedAttnArgs a) {
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, Deep, 0);
-#endif
         // element i: token tok + 8 (i / 4) + 4 h + i % 4
-        if (tok + 32 > min(low, r.t1)) {
+        if (CUT && tok + 32 > min(low, r.t1)) {
             const int seen = min(limit, r.t1) - tok - 4 * h;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -937,15 +996,17 @@ paged_many_kernel(PagedAttnArgs a) {
 #pragma unroll
         for (int i = 1; i < 16; ++i) mt = fmaxf(mt, s[i]);
         mt = fmaxf(mt, __shfl_xor(mt, 32)) * scale2;
-        const float mn = fmaxf(m, mt);
-        const float base = mn == -__builtin_inff() ? 0.0f : mn;
-        if (__ballot(mn != m) != 0) { // some row's maximum moves
-            const float alpha = exp2_f32(m - base);
+        // m follows the maximum only when that is 2^8 above it: until then the
+        // weights are at most 2^8 (and as exact), and the sums keep their scale
+        if (__ballot(mt > m + 8.0f) != 0) {
+            const float mn = fmaxf(m, mt);
+            const float alpha = exp2_f32(m - (mn == -__builtin_inff() ? 0.0f : mn));
             l *= alpha;
 #pragma unroll
             for (int j = 0; j < S::CT; ++j) acc[j] *= alpha;
             m = mn;
         }
+        const float base = m == -__builtin_inff() ? 0.0f : m;
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -953,48 +1014,70 @@ paged_many_kernel(PagedAttnArgs a) {
             sum += s[i];
         }
         l += sum;
-        if (wild) {
-            // An infinity or NaN among these tokens' V, and rows that do not
-            // see all of them: a token at a time on the vector ALU, added only
-            // where the row sees it, so that 0 times it stays out of the others.
-#pragma unroll 1
-            for (int u = 0; u < 32; ++u) {
-                float pu = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) pu = 8 * (i >> 2) + 4 * h + (i & 3) == u ? s[i] : pu;
-                pu += __shfl_xor(pu, 32); // (the other half of the lanes does not hold it)
-                if (tok + u >= limit || tok + u >= r.t1) continue;
-                const uint16_t *vu = vb + u * S::VR + 4 * h;
-#pragma unroll
-                for (int j = 0; j < S::CT; ++j)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        acc[j][i] = __builtin_fmaf(pu, low_f32<HALF>(vu[32 * j + 8 * (i >> 2) + (i & 3)]), acc[j][i]);
-            }
-            return;
-        }
         // V: lane group lane / 16 reads channels 16 (group % 2) .. of tokens 4 (group / 2) ..
         const uint16_t *vl = vb + ((lane & 15) >> 2) * S::VR + 4 * h * S::VR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) { // 16 tokens
+        auto value = [&](int k, int j) { // the operand of tokens 16 k .. and channels 32 j ..
+            const uint16_t *at = vl + 16 * k * S::VR + 32 * j;
+            const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at));
+            const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 8 * S::VR));
+            const uint2 x = __builtin_bit_cast(uint2, v0), y = __builtin_bit_cast(uint2, v1);
+            return u32x4a{x.x, x.y, y.x, y.y};
+        };
+        auto weights = [&](int k) {
             u32x4a p;
 #pragma unroll
             for (int n = 0; n < 4; ++n) p[n] = pack2<HALF>(s[8 * k + 2 * n], s[8 * k + 2 * n + 1]);
+            return p;
+        };
+        using W = Wild<HALF>;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) { // 16 tokens
+            const u32x4a p = weights(k);
 #pragma unroll
             for (int j = 0; j < S::CT; ++j) {
-                const uint16_t *at = vl + 16 * k * S::VR + 32 * j;
-                const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at));
-                const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 8 * S::VR));
-                const uint2 x = __builtin_bit_cast(uint2, v0), y = __builtin_bit_cast(uint2, v1);
-                acc[j] = mfma32<HALF>(u32x4a{x.x, x.y, y.x, y.y}, p, acc[j]);
+                u32x4a v = value(k, j);
+                if constexpr (CUT && SRC == 0) {
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) v[n] = W::without(v[n]);
+                }
+                acc[j] = mfma32<HALF>(v, p, acc[j]);
             }
         }
+        if constexpr (CUT && SRC == 0) {
+            if (!wild) return;
+            const int seen = min(limit, r.t1) - tok - 4 * h;
+#pragma unroll
+            for (int j = 0; j < S::CT; ++j)
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    f32x16 z = {};
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        u32x4a v = value(k, j), sees;
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) { // elements 8 k + 2 n and the next
+                            const int at = 8 * ((8 * k + 2 * n) >> 2) + ((2 * n) & 3);
+                            sees[n] = (at < seen ? W::One : 0u) | (at + 1 < seen ? W::One << 16 : 0u);
+                            v[n] = W::only(v[n], g != 0);
+                        }
+                        z = mfma32<HALF>(v, sees, z);
+                        __builtin_amdgcn_sched_barrier(0); // (one at a time: registers)
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) z[i] = W::reach(z[i], g != 0);
+                    acc[j] += z;
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        }
     };
-    auto work = [&](int tok, const ManyBuf<DP> &buf, bool wild) {
-#pragma unroll XUNR
+    auto work = [&](auto cut, int tok, const ManyBuf<DP> &buf, bool wild) {
+#pragma unroll 1
         for (int t = 0; t < S::ST; ++t)
-            if (t == 0 || tok + 32 * t < r.t1) work32(tok + 32 * t, buf.k + 32 * t * S::KR, buf.v + 32 * t * S::VR, wild);
+            if (!decltype(cut)::value || tok + 32 * t < r.t1)
+                work32(cut, tok + 32 * t, buf.k + 32 * t * S::KR, buf.v + 32 * t * S::VR, wild);
     };
+    using Whole = std::integral_constant<bool, false>;
+    using Cut = std::integral_constant<bool, true>;
 
     if (r.t0 < r.t1) {
         if constexpr (SRC == 0) {
@@ -1010,59 +1093,86 @@ paged_many_kernel(PagedAttnArgs a) {
             auto publish = [&](int slot) {
                 if (tid >= S::KT) return;
                 const int64_t page = held_page(a.pool, place.x, bad);
-                lds.row[slot][tid] = make_longlong2(page * a.pool.k_page + int64_t(place.y) * a.pool.k_token,
-                                                    page * a.pool.v_page + int64_t(place.y) * a.pool.v_token);
+                lds.row[slot][tid] = make_longlong2(2 * (page * a.pool.k_page + int64_t(place.y) * a.pool.k_token),
+                                                    2 * (page * a.pool.v_page + int64_t(place.y) * a.pool.v_token));
             };
-            auto request = [&](int slot, int tok) {
+            auto request = [&](int slot) {
+                const int here = thread_here();
+                const char *kc = nullptr, *vc = nullptr;
 #pragma unroll
                 for (int k = 0; k < S::NP; ++k) {
-                    const int o = tid + kPagedThreads * k, t = o / S::PR, ch = min(8 * (o - t * S::PR), a.dim - 8);
+                    const int o = here + kPagedThreads * k, t = o / S::PR;
+                    if (k == 0 || kPagedThreads % S::PR != 0) { // (else the same channels every time)
+                        const int ch = min(8 * (o - t * S::PR), a.dim - 8);
+                        kc = reinterpret_cast<const char *>(kh + ch);
+                        vc = reinterpret_cast<const char *>(vh + ch);
+                    }
                     const longlong2 at = lds.row[slot][t];
-                    kn[k] = *reinterpret_cast<const u32x4a *>(kh + (at.x + ch));
-                    vn[k] = *reinterpret_cast<const u32x4a *>(vh + (at.y + ch));
+                    kn[k] = *reinterpret_cast<const u32x4a *>(kc + at.x);
+                    vn[k] = *reinterpret_cast<const u32x4a *>(vc + at.y);
                 }
             };
             // Tokens past the split's end: V is zero. Returns whether the tile
             // holds an infinity or NaN in V where rows see different tokens of it.
             auto store = [&](ManyBuf<DP> &buf, int tok) {
                 bool w = false;
-                const bool cut = tok + S::KT > wg_low;
+                if (tok + S::KT > wg_low || tok + S::KT > r.t1) {
 #pragma unroll
-                for (int k = 0; k < S::NP; ++k) {
-                    const int o = tid + kPagedThreads * k, t = o / S::PR, ch = 8 * (o - t * S::PR);
-                    u32x4a v = vn[k];
-                    if (tok + S::KT > r.t1 && tok + t >= r.t1) v = u32x4a{0, 0, 0, 0};
-                    if (cut)
+                    for (int k = 0; k < S::NP; ++k) {
+                        const int t = (tid + kPagedThreads * k) / S::PR;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) w |= wild2<HALF>(v[i]);
-                    if (ch < a.dim) {
-                        *reinterpret_cast<u32x4a *>(buf.k + t * S::KR + ch) = kn[k];
-                        *reinterpret_cast<u32x4a *>(buf.v + t * S::VR + ch) = v;
+                        for (int i = 0; i < 4; ++i) {
+                            vn[k][i] = tok + t < r.t1 ? vn[k][i] : 0u;
+                            w |= wild2<HALF>(vn[k][i]);
+                        }
                     }
+                    w &= tok + S::KT > wg_low;
                 }
-                return cut && w;
+                const int here = thread_here();
+                auto put = [&](int k) {
+                    const int o = here + kPagedThreads * k, t = o / S::PR, ch = 8 * (o - t * S::PR);
+                    *reinterpret_cast<u32x4a *>(buf.k + t * S::KR + ch) = kn[k];
+                    *reinterpret_cast<u32x4a *>(buf.v + t * S::VR + ch) = vn[k];
+                };
+                if (a.dim == DP) {
+#pragma unroll
+                    for (int k = 0; k < S::NP; ++k) put(k);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < S::NP; ++k)
+                        if (8 * ((here + kPagedThreads * k) % S::PR) < a.dim) put(k);
+                }
+                return w;
             };
-            int tok = r.t0;
+            int tok = r.t0, b = 0;
             find(tok);
             publish(0);
             find(tok + S::KT);
             publish(1);
             find(tok + 2 * S::KT);
             __syncthreads();
-            request(0, tok);
+            request(0);
             bool w = store(lds.buf[0], tok);
-            request(1, tok + S::KT);
+            request(1);
             bool wild = __syncthreads_or(w) != 0;
-            for (int b = 0;; b ^= 1) {
-                if (busy) work(tok, lds.buf[b], wild);
-                if (tok + S::KT >= r.t1) break;
+            // works on the tile at tok and makes the next one ready; false at the end
+            auto turn = [&](auto cut) {
+                if (busy) work(cut, tok, lds.buf[b], wild);
+                if (tok + S::KT >= r.t1) return false;
                 w = store(lds.buf[b ^ 1], tok + S::KT);
                 publish(b); // the tile after next; its rows are requested after the barrier
                 find(tok + 3 * S::KT);
-                wild = __syncthreads_or(w) != 0;
+                if (tok + 2 * S::KT > wg_low) wild = __syncthreads_or(w) != 0;
+                else __syncthreads();
                 tok += S::KT;
-                if (tok + S::KT < r.t1) request(b, tok + S::KT);
-            }
+                if (tok + S::KT < r.t1) request(b);
+                b ^= 1;
+                return true;
+            };
+            // tiles that every row sees whole, then the others
+            bool more = true;
+            while (more && tok + S::KT <= min(wg_low, r.t1)) more = turn(Whole{});
+            while (more) more = turn(Cut{});
             if (bad) atomicOr(a.status, kStPage);
         } else {
             const PrefixSeg *ks = a.px[2 * head].segs, *vs = a.px[2 * head + 1].segs;
@@ -1086,7 +1196,7 @@ paged_many_kernel(PagedAttnArgs a) {
                 coded_patch<DP, S::VR>(v0, vs, a.dim, vt, lds.buf[b].v);
                 if (tok + S::KT < r.t1) request(t + 1);
                 __syncthreads();
-                if (busy) work(tok, lds.buf[b], false);
+                if (busy) work(Cut{}, tok, lds.buf[b], false);
             }
         }
     }
