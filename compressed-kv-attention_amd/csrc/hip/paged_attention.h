@@ -661,7 +661,7 @@ __device__ __forceinline__ int thread_here() {
 }
 
 // -------------------------------------------------------------- many rows --
-// Up to 128 query rows per workgroup, 32 per wave (32 x 32 x 16 products):
+// 128 or 256 query rows per workgroup, 32 per wave (32 x 32 x 16 products):
 // prompts in chunks, draft tokens, and the rows of a whole batch against a
 // shared prefix. A tile of tokens (64 up to head_dim 128, 32 above) is staged
 // in LDS, once for all rows: pages as they are, containers decoded on the way
@@ -678,8 +678,10 @@ __device__ __forceinline__ int thread_here() {
 // (containers: twice, the escapes being written over their elements between),
 // and two workgroups share a CU, so that one's products run beside the other's
 // exponentials.
-template <int DP>
+template <int DP, int NW>
 struct Many {
+    static constexpr int T = 64 * NW;                         // threads
+    static constexpr int Rows = 32 * NW;                      // query rows
     static constexpr int KT = tile_tokens(DP);
     static constexpr int ST = KT / 32;                        // score tiles
     static constexpr int KS = DP / 16;                        // steps of 16 channels
@@ -688,22 +690,22 @@ struct Many {
     static constexpr int VR = DP + (DP % 64 == 0 ? 32 : 0);   // of V: four rows 16 banks apart
     static constexpr int PR = DP / 8;                         // 16-byte pieces per row
     static constexpr int Occ = DP <= 128 ? 2 : 1;             // waves per SIMD that the registers allow
-    static constexpr int NP = KT * PR / kPagedThreads;        // pieces per thread (pages)
-    static_assert(KT * PR % kPagedThreads == 0, "whole pieces per thread");
+    static constexpr int Pieces = KT * PR;
+    static constexpr int NP = (Pieces + T - 1) / T;           // pieces per thread (pages)
     // containers: a thread keeps to one column of 8 channels, RP rows a pass
-    static constexpr int RP = kPagedThreads / PR;
+    static constexpr int RP = T / PR < KT ? T / PR : KT;
     static constexpr int NR = (KT + RP - 1) / RP;
 };
 
 template <int DP>
 struct alignas(16) ManyBuf {
-    uint16_t k[Many<DP>::KT * Many<DP>::KR];
-    uint16_t v[Many<DP>::KT * Many<DP>::VR];
+    uint16_t k[Many<DP, 4>::KT * Many<DP, 4>::KR];
+    uint16_t v[Many<DP, 4>::KT * Many<DP, 4>::VR];
 };
 template <int DP>
 struct alignas(16) ManyLds {
     ManyBuf<DP> buf[2];
-    longlong2 row[2][Many<DP>::KT]; // where K and V of the tokens of tiles on their way begin (bytes)
+    longlong2 row[2][Many<DP, 4>::KT]; // where K and V of the tokens of tiles on their way begin (bytes)
 };
 
 typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
@@ -784,9 +786,9 @@ __device__ __forceinline__ void base_words(uint2 base, uint32_t (&bp)[4]) {
 // A tile of a container tensor on its way: the rows of its first run in
 // registers (pass k: row RP k + the thread's row), and its first escape
 // records, one per thread.
-template <int DP>
+template <int DP, int NW>
 struct CodedTile {
-    CodedOctet o[Many<DP>::NR];
+    CodedOctet o[Many<DP, NW>::NR];
     uint2 base;
     uint32_t rec;
 };
@@ -798,29 +800,30 @@ struct Column {
 
 // Whether a run fills the tile and its rows the passes (the usual case): then a
 // pass is a fixed step of the streams after the one before.
-template <int DP>
+template <int DP, int NW>
 __device__ __forceinline__ bool whole_run(const PrefixSeg &s, int dim) {
-    return s.rows == Many<DP>::KT && dim == DP && kPagedThreads % Many<DP>::PR == 0;
+    using S = Many<DP, NW>;
+    return s.rows == S::KT && dim == DP && S::T % S::PR == 0 && S::T <= S::Pieces;
 }
 
-template <int DP>
-__device__ __forceinline__ void coded_load(const PrefixSeg &s, int dim, const Column &at, CodedTile<DP> &t) {
-    using S = Many<DP>;
+template <int DP, int NW>
+__device__ __forceinline__ void coded_load(const PrefixSeg &s, int dim, const Column &at, CodedTile<DP, NW> &t) {
+    using S = Many<DP, NW>;
     const int tid = thread_here();
     t.rec = s.esc[max(min(tid, s.n_esc - 1), 0)];
     // (a plain block has no base exponents; it starts with at least a row)
     const any_u32x2 b = *reinterpret_cast<const any_u32x2 *>(s.data + uint32_t(at.ch));
     t.base = make_uint2(b.x, b.y);
-    if (s.mode != 0 && whole_run<DP>(s, dim)) {
+    if (s.mode != 0 && whole_run<DP, NW>(s, dim)) {
         const uint32_t e0 = uint32_t(8 * tid); // element of the run
         const uint8_t *sm = s.data + (DP + s.row0 * DP),
                       *codes = s.data + (DP + s.n_tokens * DP + s.row0 * (DP / 8) * s.mode + s.mode - 4);
         const uint32_t c0 = uint32_t(tid) * uint32_t(s.mode);
 #pragma unroll
         for (int k = 0; k < S::NR; ++k) {
-            const any_u32x2 x = *reinterpret_cast<const any_u32x2 *>(sm + 8 * kPagedThreads * k + e0);
+            const any_u32x2 x = *reinterpret_cast<const any_u32x2 *>(sm + 8 * S::T * k + e0);
             t.o[k].sm = make_uint2(x.x, x.y);
-            t.o[k].c = make_uint2(*reinterpret_cast<const any_u32 *>(codes + kPagedThreads * k * s.mode + c0), 0);
+            t.o[k].c = make_uint2(*reinterpret_cast<const any_u32 *>(codes + S::T * k * s.mode + c0), 0);
         }
         return;
     }
@@ -836,14 +839,14 @@ __device__ __forceinline__ void coded_load(const PrefixSeg &s, int dim, const Co
 
 // The run's rows to LDS rows of R elements; V: the tile's other rows are zero
 // (a run of the tile's end: the prefix's end) before further runs are written.
-template <int DP, int R, bool V>
+template <int DP, int NW, int R, bool V>
 __device__ __forceinline__ void coded_store(const PrefixSeg &s, const PrefixSeg *segs, int dim, const Column &at,
-                                            const CodedTile<DP> &t, uint16_t *lds) {
-    using S = Many<DP>;
+                                            const CodedTile<DP, NW> &t, uint16_t *lds) {
+    using S = Many<DP, NW>;
     const uint32_t smm = wave::sm_mask_vgpr();
     const bool mine = at.row < at.step; // (threads past the whole rows of a pass have none)
     auto put = [&](auto octet) {
-        if (whole_run<DP>(s, dim)) {
+        if (whole_run<DP, NW>(s, dim)) {
             uint16_t *to = lds + at.row * R + at.ch;
 #pragma unroll
             for (int k = 0; k < S::NR; ++k) *reinterpret_cast<u32x4a *>(to + k * S::RP * R) = octet(k);
@@ -898,40 +901,41 @@ __device__ __forceinline__ void patch_one(const PrefixSeg &s, int dim, uint32_t 
     if (uint32_t(row) < uint32_t(s.rows)) // (a damaged container's records)
         lds[(s.dst + row) * R + octet_place(e - (row + s.row0) * dim)] = uint16_t(rec >> 16);
 }
-template <int DP, int R>
-__device__ __forceinline__ void coded_patch(const PrefixSeg &s, const PrefixSeg *segs, int dim, const CodedTile<DP> &t,
+template <int DP, int NW, int R>
+__device__ __forceinline__ void coded_patch(const PrefixSeg &s, const PrefixSeg *segs, int dim,
+                                            const CodedTile<DP, NW> &t,
                                             uint16_t *lds) {
     const int tid = int(threadIdx.x);
     if (tid < s.n_esc) patch_one<R>(s, dim, t.rec, lds);
-    for (int i = tid + kPagedThreads; i < s.n_esc; i += kPagedThreads) patch_one<R>(s, dim, s.esc[i], lds);
+    for (int i = tid + 64 * NW; i < s.n_esc; i += 64 * NW) patch_one<R>(s, dim, s.esc[i], lds);
     for (int k = 0; k < s.n_more; ++k) {
         const PrefixSeg g = seg_at(segs, s.more + k);
-        for (int i = tid; i < g.n_esc; i += kPagedThreads) patch_one<R>(g, dim, g.esc[i], lds);
+        for (int i = tid; i < g.n_esc; i += 64 * NW) patch_one<R>(g, dim, g.esc[i], lds);
     }
 }
 
-template <int DP, bool HALF, int SRC>
-__global__ __launch_bounds__(kPagedThreads) __attribute__((amdgpu_waves_per_eu(Many<DP>::Occ, Many<DP>::Occ))) void
+template <int DP, bool HALF, int SRC, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(Many<DP, NW>::Occ, Many<DP, NW>::Occ))) void
 paged_many_kernel(PagedAttnArgs a) {
-    using S = Many<DP>;
+    using S = Many<DP, NW>;
     extern __shared__ __align__(16) uint8_t many_lds[];
     ManyLds<DP> &lds = *reinterpret_cast<ManyLds<DP> *>(many_lds);
     const int tid = int(threadIdx.x), lane = lane_id(), wave = tid >> 6, c = lane & 31, h = lane >> 5;
     int split, head, tile, seq;
     find_work(a, split, head, tile, seq);
     Rows r;
-    find_rows(a, seq, split, tile, 32 * kPagedWaves, r);
-    if (32 * kPagedWaves * tile >= r.count || !r.used) return;
-    const int r0 = 32 * (kPagedWaves * tile + wave);
+    find_rows(a, seq, split, tile, S::Rows, r);
+    if (S::Rows * tile >= r.count || !r.used) return;
+    const int r0 = 32 * (NW * tile + wave);
     const int row = r0 + c, limit = row_limit(a, r, row);
     const bool busy = r0 < r.count;
     const int low = row_limit(a, r, min(r0, r.count - 1)); // the wave's fewest tokens
-    const int wg_low = row_limit(a, r, 32 * kPagedWaves * tile);
+    const int wg_low = row_limit(a, r, S::Rows * tile);
     const int32_t *table = a.batch.table + (a.shared ? 0 : int64_t(seq) * a.batch.table_stride);
     const uint16_t *kh = a.pool.k + int64_t(head) * a.pool.k_head;
     const uint16_t *vh = a.pool.v + int64_t(head) * a.pool.v_head;
     // channels past head_dim: K's are zero (they meet zero queries), V's feed outputs that nobody reads
-    for (int i = tid; i < 2 * S::KT * (DP - a.dim); i += kPagedThreads) {
+    for (int i = tid; i < 2 * S::KT * (DP - a.dim); i += S::T) {
         const int t = i / (DP - a.dim), d = a.dim + i - t * (DP - a.dim), b = t / S::KT;
         lds.buf[b].k[(t - b * S::KT) * S::KR + d] = 0;
         lds.buf[b].v[(t - b * S::KT) * S::VR + d] = 0;
@@ -964,37 +968,44 @@ paged_many_kernel(PagedAttnArgs a) {
         for (int i = 0; i < 16; ++i) acc[j][i] = 0.0f;
     float m = -__builtin_inff(), l = 0.0f;
 
-    // ---- 32 tokens of a tile, from its half of LDS
-    // (CUT: some row of the workgroup does not see all of the tile)
-    auto work32 = [&](auto cut, int tok, const uint16_t *kb, const uint16_t *vb, bool wild) {
+    // ---- one tile, from its half of LDS (CUT: some row of the workgroup does
+    // not see all of it). All its scores first: one maximum, one branch, and
+    // the second half's exponentials run beside the first half's products.
+    auto work = [&](auto cut, int tok, const ManyBuf<DP> &buf, bool wild) {
         constexpr bool CUT = decltype(cut)::value;
-        f32x16 s;
+        f32x16 s[S::ST];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+        for (int t = 0; t < S::ST; ++t) {
+            s[t] = f32x16{};
 #pragma unroll
-        for (int i = 0; i < S::KS; ++i) {
-            const u32x4a kf = *reinterpret_cast<const u32x4a *>(kb + c * S::KR + 16 * i + 8 * h);
-            s = mfma32<HALF>(kf, q[i], s);
+            for (int i = 0; i < S::KS; ++i) {
+                const u32x4a kf = *reinterpret_cast<const u32x4a *>(buf.k + (32 * t + c) * S::KR + 16 * i + 8 * h);
+                s[t] = mfma32<HALF>(kf, q[i], s[t]);
+            }
         }
         // a few rows of K ahead of the products (else each product waits for its own)
-        constexpr int Deep = S::KS < 4 ? S::KS : 4;
+        constexpr int Reads = S::KS * S::ST, Deep = Reads < 6 ? Reads : 6;
         __builtin_amdgcn_sched_group_barrier(0x100, Deep, 0);
 #pragma unroll
-        for (int i = 0; i < S::KS - Deep; ++i) {
+        for (int i = 0; i < Reads - Deep; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, Deep, 0);
-        // element i: token tok + 8 (i / 4) + 4 h + i % 4
-        if (CUT && tok + 32 > min(low, r.t1)) {
+        // element i of s[t]: token tok + 32 t + 8 (i / 4) + 4 h + i % 4
+        if (CUT && tok + S::KT > min(low, r.t1)) {
             const int seen = min(limit, r.t1) - tok - 4 * h;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (8 * (i >> 2) + (i & 3) >= seen) s[i] = -__builtin_inff();
-        }
-        float mt = s[0];
+            for (int t = 0; t < S::ST; ++t)
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mt = fmaxf(mt, s[i]);
+                for (int i = 0; i < 16; ++i)
+                    if (32 * t + 8 * (i >> 2) + (i & 3) >= seen) s[t][i] = -__builtin_inff();
+        }
+        float mt = s[0][0];
+#pragma unroll
+        for (int t = 0; t < S::ST; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[t][i]);
         mt = fmaxf(mt, __shfl_xor(mt, 32)) * scale2;
         // m follows the maximum only when that is 2^8 above it: until then the
         // weights are at most 2^8 (and as exact), and the sums keep their scale
@@ -1007,15 +1018,8 @@ paged_many_kernel(PagedAttnArgs a) {
             m = mn;
         }
         const float base = m == -__builtin_inff() ? 0.0f : m;
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[i] = exp2_f32(__builtin_fmaf(s[i], scale2, -base));
-            sum += s[i];
-        }
-        l += sum;
         // V: lane group lane / 16 reads channels 16 (group % 2) .. of tokens 4 (group / 2) ..
-        const uint16_t *vl = vb + ((lane & 15) >> 2) * S::VR + 4 * h * S::VR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        const uint16_t *vl = buf.v + ((lane & 15) >> 2) * S::VR + 4 * h * S::VR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
         auto value = [&](int k, int j) { // the operand of tokens 16 k .. and channels 32 j ..
             const uint16_t *at = vl + 16 * k * S::VR + 32 * j;
             const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at));
@@ -1023,16 +1027,21 @@ paged_many_kernel(PagedAttnArgs a) {
             const uint2 x = __builtin_bit_cast(uint2, v0), y = __builtin_bit_cast(uint2, v1);
             return u32x4a{x.x, x.y, y.x, y.y};
         };
-        auto weights = [&](int k) {
+        using W = Wild<HALF>;
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < 2 * S::ST; ++k) { // 16 tokens
+            f32x16 &sk = s[k >> 1];
             u32x4a p;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) p[n] = pack2<HALF>(s[8 * k + 2 * n], s[8 * k + 2 * n + 1]);
-            return p;
-        };
-        using W = Wild<HALF>;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) { // 16 tokens
-            const u32x4a p = weights(k);
+            for (int n = 0; n < 4; ++n) {
+                const int i = 8 * (k & 1) + 2 * n;
+                const float p0 = exp2_f32(__builtin_fmaf(sk[i], scale2, -base)),
+                            p1 = exp2_f32(__builtin_fmaf(sk[i + 1], scale2, -base));
+                sum[0] += p0;
+                sum[1] += p1;
+                p[n] = pack2<HALF>(p0, p1);
+            }
 #pragma unroll
             for (int j = 0; j < S::CT; ++j) {
                 u32x4a v = value(k, j);
@@ -1043,6 +1052,7 @@ paged_many_kernel(PagedAttnArgs a) {
                 acc[j] = mfma32<HALF>(v, p, acc[j]);
             }
         }
+        l += sum[0] + sum[1];
         if constexpr (CUT && SRC == 0) {
             if (!wild) return;
             const int seen = min(limit, r.t1) - tok - 4 * h;
@@ -1052,11 +1062,11 @@ paged_many_kernel(PagedAttnArgs a) {
                 for (int g = 0; g < 2; ++g) {
                     f32x16 z = {};
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
+                    for (int k = 0; k < 2 * S::ST; ++k) {
                         u32x4a v = value(k, j), sees;
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) { // elements 8 k + 2 n and the next
-                            const int at = 8 * ((8 * k + 2 * n) >> 2) + ((2 * n) & 3);
+                        for (int n = 0; n < 4; ++n) { // tokens at and at + 1 of the tile (plus 4 h)
+                            const int at = 16 * k + 8 * (n >> 1) + ((2 * n) & 3);
                             sees[n] = (at < seen ? W::One : 0u) | (at + 1 < seen ? W::One << 16 : 0u);
                             v[n] = W::only(v[n], g != 0);
                         }
@@ -1069,12 +1079,6 @@ paged_many_kernel(PagedAttnArgs a) {
                     __builtin_amdgcn_sched_barrier(0);
                 }
         }
-    };
-    auto work = [&](auto cut, int tok, const ManyBuf<DP> &buf, bool wild) {
-#pragma unroll 1
-        for (int t = 0; t < S::ST; ++t)
-            if (!decltype(cut)::value || tok + 32 * t < r.t1)
-                work32(cut, tok + 32 * t, buf.k + 32 * t * S::KR, buf.v + 32 * t * S::VR, wild);
     };
     using Whole = std::integral_constant<bool, false>;
     using Cut = std::integral_constant<bool, true>;
@@ -1101,8 +1105,8 @@ paged_many_kernel(PagedAttnArgs a) {
                 const char *kc = nullptr, *vc = nullptr;
 #pragma unroll
                 for (int k = 0; k < S::NP; ++k) {
-                    const int o = here + kPagedThreads * k, t = o / S::PR;
-                    if (k == 0 || kPagedThreads % S::PR != 0) { // (else the same channels every time)
+                    const int o = min(here + S::T * k, S::Pieces - 1), t = o / S::PR;
+                    if (k == 0 || S::T % S::PR != 0) { // (else the same channels every time)
                         const int ch = min(8 * (o - t * S::PR), a.dim - 8);
                         kc = reinterpret_cast<const char *>(kh + ch);
                         vc = reinterpret_cast<const char *>(vh + ch);
@@ -1119,7 +1123,7 @@ paged_many_kernel(PagedAttnArgs a) {
                 if (tok + S::KT > wg_low || tok + S::KT > r.t1) {
 #pragma unroll
                     for (int k = 0; k < S::NP; ++k) {
-                        const int t = (tid + kPagedThreads * k) / S::PR;
+                        const int t = (tid + S::T * k) / S::PR;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             vn[k][i] = tok + t < r.t1 ? vn[k][i] : 0u;
@@ -1130,7 +1134,8 @@ paged_many_kernel(PagedAttnArgs a) {
                 }
                 const int here = thread_here();
                 auto put = [&](int k) {
-                    const int o = here + kPagedThreads * k, t = o / S::PR, ch = 8 * (o - t * S::PR);
+                    const int o = here + S::T * k, t = o / S::PR, ch = 8 * (o - t * S::PR);
+                    if (S::Pieces % S::T != 0 && o >= S::Pieces) return;
                     *reinterpret_cast<u32x4a *>(buf.k + t * S::KR + ch) = kn[k];
                     *reinterpret_cast<u32x4a *>(buf.v + t * S::VR + ch) = vn[k];
                 };
@@ -1140,7 +1145,7 @@ paged_many_kernel(PagedAttnArgs a) {
                 } else {
 #pragma unroll
                     for (int k = 0; k < S::NP; ++k)
-                        if (8 * ((here + kPagedThreads * k) % S::PR) < a.dim) put(k);
+                        if (8 * ((here + S::T * k) % S::PR) < a.dim) put(k);
                 }
                 return w;
             };
@@ -1163,7 +1168,7 @@ paged_many_kernel(PagedAttnArgs a) {
                 publish(b); // the tile after next; its rows are requested after the barrier
                 find(tok + 3 * S::KT);
                 if (tok + 2 * S::KT > wg_low) wild = __syncthreads_or(w) != 0;
-                else __syncthreads();
+                else team::team_sync(); // (the loads on their way stay on their way)
                 tok += S::KT;
                 if (tok + S::KT < r.t1) request(b);
                 b ^= 1;
@@ -1177,25 +1182,31 @@ paged_many_kernel(PagedAttnArgs a) {
         } else {
             const PrefixSeg *ks = a.px[2 * head].segs, *vs = a.px[2 * head + 1].segs;
             const int pr = a.dim / 8, last = (r.len - 1) / S::KT;
-            const Column at{8 * (tid % pr), tid / pr, kPagedThreads / pr};
-            CodedTile<DP> kt, vt;
-            PrefixSeg k0, v0; // the tile's first runs
+            const Column at{8 * (tid % pr), tid / pr, min(S::T / pr, S::KT)};
+            CodedTile<DP, NW> kt, vt;
+            // the tile's first runs, and the next tile's on their way (a run's
+            // loads would wait for it)
+            PrefixSeg k0, v0, k1, v1;
             auto request = [&](int t) {
-                k0 = seg_at(ks, min(t, last));
-                v0 = seg_at(vs, min(t, last));
-                coded_load<DP>(k0, a.dim, at, kt);
-                coded_load<DP>(v0, a.dim, at, vt);
+                k0 = k1;
+                v0 = v1;
+                coded_load<DP, NW>(k0, a.dim, at, kt);
+                coded_load<DP, NW>(v0, a.dim, at, vt);
+                k1 = seg_at(ks, min(t + 1, last));
+                v1 = seg_at(vs, min(t + 1, last));
             };
             int t = r.t0 / S::KT;
+            k1 = seg_at(ks, min(t, last));
+            v1 = seg_at(vs, min(t, last));
             request(t);
             for (int tok = r.t0, b = 0; tok < r.t1; tok += S::KT, ++t, b ^= 1) {
-                coded_store<DP, S::KR, false>(k0, ks, a.dim, at, kt, lds.buf[b].k);
-                coded_store<DP, S::VR, true>(v0, vs, a.dim, at, vt, lds.buf[b].v);
-                __syncthreads();
-                coded_patch<DP, S::KR>(k0, ks, a.dim, kt, lds.buf[b].k);
-                coded_patch<DP, S::VR>(v0, vs, a.dim, vt, lds.buf[b].v);
+                coded_store<DP, NW, S::KR, false>(k0, ks, a.dim, at, kt, lds.buf[b].k);
+                coded_store<DP, NW, S::VR, true>(v0, vs, a.dim, at, vt, lds.buf[b].v);
+                team::team_sync(); // (as below: loads on their way stay on their way)
+                coded_patch<DP, NW, S::KR>(k0, ks, a.dim, kt, lds.buf[b].k);
+                coded_patch<DP, NW, S::VR>(v0, vs, a.dim, vt, lds.buf[b].v);
                 if (tok + S::KT < r.t1) request(t + 1);
-                __syncthreads();
+                team::team_sync();
                 if (busy) work(Cut{}, tok, lds.buf[b], false);
             }
         }

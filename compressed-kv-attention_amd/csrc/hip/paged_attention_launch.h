@@ -27,22 +27,29 @@ void launch_few(const PagedAttnArgs &a, bool two, int n_seqs, hipStream_t s) {
     halves ? launch_few_c<DP, HALF, 1, true>(a, n_seqs, s) : launch_few_c<DP, HALF, 1, false>(a, n_seqs, s);
 }
 
-template <int DP, bool HALF, int SRC>
-hipError_t launch_many_src(const PagedAttnArgs &a, int n_seqs, hipStream_t s) {
+template <int DP, bool HALF, int SRC, int NW>
+hipError_t launch_many_waves(const PagedAttnArgs &a, int n_seqs, hipStream_t s) {
     // (past the default 64 KiB of LDS at some sizes; set once per instantiation)
     static const hipError_t set =
-        hipFuncSetAttribute(reinterpret_cast<const void *>(paged_many_kernel<DP, HALF, SRC>),
+        hipFuncSetAttribute(reinterpret_cast<const void *>(paged_many_kernel<DP, HALF, SRC, NW>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(ManyLds<DP>)));
     if (set != hipSuccess) return set;
-    hipLaunchKernelGGL((paged_many_kernel<DP, HALF, SRC>), attention_grid(a, n_seqs), dim3(kPagedThreads),
+    hipLaunchKernelGGL((paged_many_kernel<DP, HALF, SRC, NW>), attention_grid(a, n_seqs), dim3(64 * NW),
                        sizeof(ManyLds<DP>), s, a);
     return hipGetLastError();
 }
 
+template <int DP, bool HALF, int SRC>
+hipError_t launch_many_src(const PagedAttnArgs &a, int tile_rows, int n_seqs, hipStream_t s) {
+    if constexpr (many_rows(DP) == 256)
+        if (tile_rows == 256) return launch_many_waves<DP, HALF, SRC, 8>(a, n_seqs, s);
+    return launch_many_waves<DP, HALF, SRC, 4>(a, n_seqs, s);
+}
+
 template <int DP>
-hipError_t launch_many(const PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s) {
-    if (a.px != nullptr) return launch_many_src<DP, false, 1>(a, n_seqs, s);
-    return half ? launch_many_src<DP, true, 0>(a, n_seqs, s) : launch_many_src<DP, false, 0>(a, n_seqs, s);
+hipError_t launch_many(const PagedAttnArgs &a, bool half, int tile_rows, int n_seqs, hipStream_t s) {
+    if (a.px != nullptr) return launch_many_src<DP, false, 1>(a, tile_rows, n_seqs, s);
+    return half ? launch_many_src<DP, true, 0>(a, tile_rows, n_seqs, s) : launch_many_src<DP, false, 0>(a, tile_rows, n_seqs, s);
 }
 
 } // namespace paged
@@ -54,6 +61,7 @@ hipError_t launch_many(const PagedAttnArgs &a, bool half, int n_seqs, hipStream_
         else kvexp_dev::paged::launch_few<DP, false>(a, two, n_seqs, s);                                              \
         return hipGetLastError();                                                                                     \
     }                                                                                                                 \
-    hipError_t paged_many_d##DP(const kvexp_dev::PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s) {            \
-        return kvexp_dev::paged::launch_many<DP>(a, half, n_seqs, s);                                                 \
+    hipError_t paged_many_d##DP(const kvexp_dev::PagedAttnArgs &a, bool half, int tile_rows, int n_seqs,         \
+                                 hipStream_t s) {                                                                     \
+        return kvexp_dev::paged::launch_many<DP>(a, half, tile_rows, n_seqs, s);                                      \
     }

@@ -162,7 +162,7 @@ using namespace kvexp_dev;
 
 #define KVEXP_PAGED_DECL(DP)                                                                       \
     hipError_t paged_few_d##DP(const PagedAttnArgs &a, bool half, bool two, int n_seqs, hipStream_t s); \
-    hipError_t paged_many_d##DP(const PagedAttnArgs &a, bool half, int n_seqs, hipStream_t s);
+    hipError_t paged_many_d##DP(const PagedAttnArgs &a, bool half, int tile_rows, int n_seqs, hipStream_t s);
 KVEXP_PAGED_DECL(32)
 KVEXP_PAGED_DECL(64)
 KVEXP_PAGED_DECL(96)
@@ -170,11 +170,11 @@ KVEXP_PAGED_DECL(128)
 KVEXP_PAGED_DECL(192)
 KVEXP_PAGED_DECL(256)
 
-// tile_rows: 16 or 32 (the few-row kernel), or the many-row kernel's.
+// tile_rows: 16 or 32 (the few-row kernel), 128 or 256 (the many-row kernel).
 hipError_t paged_attention(const PagedAttnArgs &a, bool half, int tile_rows, int n_seqs, hipStream_t s) {
     const bool many = tile_rows > 32, two = tile_rows == 32;
 #define KVEXP_PAGED_PICK(DP) \
-    if (a.dim <= DP) return many ? paged_many_d##DP(a, half, n_seqs, s) : paged_few_d##DP(a, half, two, n_seqs, s);
+    if (a.dim <= DP) return many ? paged_many_d##DP(a, half, tile_rows, n_seqs, s) : paged_few_d##DP(a, half, two, n_seqs, s);
     KVEXP_PAGED_PICK(32)
     KVEXP_PAGED_PICK(64)
     KVEXP_PAGED_PICK(96)

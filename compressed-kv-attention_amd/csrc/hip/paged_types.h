@@ -124,6 +124,9 @@ constexpr int tile_tokens(int dim) { return dim <= 128 ? 64 : 32; }
 // Query rows of a workgroup of the few-row kernel, at most: 16, or 32 in two
 // products where the registers hold them.
 constexpr int few_rows(int dim) { return dim <= 128 ? 32 : 16; }
+// Of the many-row kernel, at most: 128, or 256 where eight waves' registers
+// hold the outputs.
+constexpr int many_rows(int dim) { return dim <= 192 ? 256 : 128; }
 template <int DP>
 constexpr int kFewRowsAt = few_rows(DP);
 

@@ -6,6 +6,9 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#ifndef XROWS
+#define XROWS 128
+#endif
 #include <cstring>
 
 #include "../hip/paged_types.h"
@@ -31,7 +34,6 @@ namespace {
 
 constexpr int kMaxHeadDim = 256;
 constexpr int64_t kGridMax = (int64_t(1) << 24) - 1; // workgroups of 256 threads below 2^32 threads
-constexpr int kManyRows = 128;
 
 [[noreturn]] void bad(const std::string &msg) { fail(KVEXP_HIP_INVALID_ARGUMENT, msg); }
 
@@ -159,10 +161,10 @@ Cut cut_of(const kvexp_hip_ctx *ctx, int64_t rows, int64_t pairs, int max_len, i
     if (rows > INT32_MAX / 2) fail(KVEXP_HIP_UNSUPPORTED, "paged attention: too many query rows");
     c.rows = int(rows);
     const bool many = coded || rows > few_rows(dim);
-    c.tile_rows = many ? kManyRows : rows > 16 ? 32 : 16;
+    c.tile_rows = !many ? (rows > 16 ? 32 : 16) : rows > XROWS ? many_rows(dim) : 128;
     c.row_tiles = int((rows + c.tile_rows - 1) / c.tile_rows);
     c.min_split = 256;
-    const int64_t target = int64_t(std::max(1, ctx->cu_count)) * (many ? 2 : 8);
+    const int64_t target = int64_t(std::max(1, ctx->cu_count)) * (many ? (c.tile_rows == 256 ? 1 : 2) : 8);
     const int64_t base = std::max<int64_t>(1, pairs * c.row_tiles);
     const int64_t most = std::max<int64_t>(1, (int64_t(max_len) + c.min_split - 1) / c.min_split);
     c.n_splits = int(std::max<int64_t>(1, std::min<int64_t>({(target + base - 1) / base, most, 256})));
