@@ -41,7 +41,7 @@ hipError_t launch_many_waves(const PagedAttnArgs &a, int n_seqs, hipStream_t s) 
 
 template <int DP, bool HALF, int SRC>
 hipError_t launch_many_src(const PagedAttnArgs &a, int tile_rows, int n_seqs, hipStream_t s) {
-    if constexpr (many_rows(DP) == 256)
+    if constexpr (many_rows(DP, SRC == 1) == 256)
         if (tile_rows == 256) return launch_many_waves<DP, HALF, SRC, 8>(a, n_seqs, s);
     return launch_many_waves<DP, HALF, SRC, 4>(a, n_seqs, s);
 }

@@ -125,8 +125,8 @@ constexpr int tile_tokens(int dim) { return dim <= 128 ? 64 : 32; }
 // products where the registers hold them.
 constexpr int few_rows(int dim) { return dim <= 128 ? 32 : 16; }
 // Of the many-row kernel, at most: 128, or 256 where eight waves' registers
-// hold the outputs.
-constexpr int many_rows(int dim) { return dim <= 192 ? 256 : 128; }
+// hold the outputs (and, for containers, the coded rows on their way).
+constexpr int many_rows(int dim, bool coded) { return dim <= (coded ? 128 : 192) ? 256 : 128; }
 template <int DP>
 constexpr int kFewRowsAt = few_rows(DP);
 

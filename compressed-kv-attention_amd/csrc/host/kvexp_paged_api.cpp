@@ -161,13 +161,15 @@ Cut cut_of(const kvexp_hip_ctx *ctx, int64_t rows, int64_t pairs, int max_len, i
     if (rows > INT32_MAX / 2) fail(KVEXP_HIP_UNSUPPORTED, "paged attention: too many query rows");
     c.rows = int(rows);
     const bool many = coded || rows > few_rows(dim);
-    c.tile_rows = !many ? (rows > 16 ? 32 : 16) : rows > XROWS ? many_rows(dim) : 128;
+    c.tile_rows = !many ? (rows > 16 ? 32 : 16) : rows > XROWS ? many_rows(dim, coded) : 128;
     c.row_tiles = int((rows + c.tile_rows - 1) / c.tile_rows);
     c.min_split = 256;
     const int64_t target = int64_t(std::max(1, ctx->cu_count)) * (many ? (c.tile_rows == 256 ? 1 : 2) : 8);
     const int64_t base = std::max<int64_t>(1, pairs * c.row_tiles);
+    // (many rows: the workgroups that are resident, no second round for a few more)
+    const int64_t want = many ? std::max<int64_t>(1, target / base) : (target + base - 1) / base;
     const int64_t most = std::max<int64_t>(1, (int64_t(max_len) + c.min_split - 1) / c.min_split);
-    c.n_splits = int(std::max<int64_t>(1, std::min<int64_t>({(target + base - 1) / base, most, 256})));
+    c.n_splits = int(std::max<int64_t>(1, std::min<int64_t>({want, most, 256})));
     // the splits of the longest sequence the call may hold: shorter ones take fewer
     const int64_t even = (int64_t(max_len) + c.n_splits - 1) / c.n_splits;
     c.min_split = int(std::max<int64_t>(c.min_split, (even + 63) / 64 * 64));
