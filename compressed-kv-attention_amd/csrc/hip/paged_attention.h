@@ -203,7 +203,7 @@ __device__ __forceinline__ int page_at(const PagedAttnArgs &a, const int32_t *ta
 
 // The state slot of a row and split.
 __device__ __forceinline__ int64_t state_slot(const PagedAttnArgs &a, const Rows &r, int head, int split, int row) {
-    return ((int64_t(r.seq) * a.n_kv + head) * a.n_splits + split) * a.max_rows + row;
+    return (int64_t(head) * a.n_splits + split) * a.max_rows + int64_t(r.first) * a.group + row;
 }
 
 // The sums of a row that saw l 0 are nothing: its output is 0.
@@ -711,7 +711,14 @@ struct alignas(16) ManyLds {
 typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
 typedef uint32_t any_u32x2 __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t any_u32 __attribute__((aligned(1)));
-typedef uint16_t any_u16 __attribute__((aligned(1)));
+
+// A load from global memory at any alignment. (A pointer that comes from lanes
+// says nothing of where it points; a flat load would count as an LDS access too,
+// and the barriers would wait for it.)
+template <class T>
+__device__ __forceinline__ T global_at(const void *p) {
+    return *(const __attribute__((address_space(1))) T *)(uintptr_t)(p);
+}
 
 // An octet of channels of a coded tensor is kept in LDS as the decoder of the
 // decode kernels gives it: dword p holds channels p and p + 4. The queries are
@@ -758,16 +765,16 @@ __device__ __forceinline__ PrefixSeg seg_of(uint32_t w) {
 __device__ __forceinline__ void load_octet(const PrefixSeg &s, bool plain, int dim, int row, int ch, CodedOctet &o) {
     const uint32_t e = uint32_t((s.row0 + row) * dim + ch); // element of the block
     if (plain) {
-        const any_u32x2 a = *reinterpret_cast<const any_u32x2 *>(s.data + 2 * e),
-                        b = *reinterpret_cast<const any_u32x2 *>(s.data + (2 * e + 8));
+        const any_u32x2 a = global_at<any_u32x2>(s.data + 2 * e),
+                        b = global_at<any_u32x2>(s.data + (2 * e + 8));
         o.sm = make_uint2(a.x, a.y);
         o.c = make_uint2(b.x, b.y);
         return;
     }
-    const any_u32x2 sm = *reinterpret_cast<const any_u32x2 *>(s.data + (uint32_t(dim) + e));
+    const any_u32x2 sm = global_at<any_u32x2>(s.data + (uint32_t(dim) + e));
     o.sm = make_uint2(sm.x, sm.y);
     const uint8_t *codes = s.data + (dim + s.n_tokens * dim + s.mode - 4);
-    o.c = make_uint2(*reinterpret_cast<const any_u32 *>(codes + (e >> 3) * uint32_t(s.mode)), 0);
+    o.c = make_uint2(global_at<any_u32>(codes + (e >> 3) * uint32_t(s.mode)), 0);
 }
 
 // The octet's BF16 words in octet order (escapes come after), from its base
@@ -819,9 +826,9 @@ template <int DP, int NW>
 __device__ __forceinline__ void coded_load(const PrefixSeg &s, int dim, const Column &at, CodedTile<DP, NW> &t) {
     using S = Many<DP, NW>;
     const int tid = thread_here();
-    t.rec = s.esc[max(min(tid, s.n_esc - 1), 0)];
+    t.rec = global_at<uint32_t>(s.esc + max(min(tid, s.n_esc - 1), 0));
     // (a plain block has no base exponents; it starts with at least a row)
-    const any_u32x2 b = *reinterpret_cast<const any_u32x2 *>(s.data + uint32_t(at.ch));
+    const any_u32x2 b = global_at<any_u32x2>(s.data + uint32_t(at.ch));
     t.base = make_uint2(b.x, b.y);
     if (s.mode != 0 && whole_run<DP, NW>(s, dim)) {
         const uint32_t e0 = uint32_t(8 * tid); // element of the run
@@ -830,9 +837,9 @@ __device__ __forceinline__ void coded_load(const PrefixSeg &s, int dim, const Co
         const uint32_t c0 = uint32_t(tid) * uint32_t(s.mode);
 #pragma unroll
         for (int k = 0; k < S::NR; ++k) {
-            const any_u32x2 x = *reinterpret_cast<const any_u32x2 *>(sm + 8 * S::T * k + e0);
+            const any_u32x2 x = global_at<any_u32x2>(sm + 8 * S::T * k + e0);
             t.o[k].sm = make_uint2(x.x, x.y);
-            t.o[k].c = make_uint2(*reinterpret_cast<const any_u32 *>(codes + S::T * k * s.mode + c0), 0);
+            t.o[k].c = make_uint2(global_at<any_u32>(codes + S::T * k * s.mode + c0), 0);
         }
         return;
     }
@@ -884,7 +891,7 @@ __device__ __forceinline__ void coded_store(const PrefixSeg &s, const PrefixSeg 
         end = g.dst + g.rows;
         uint2 base = make_uint2(0, 0);
         if (g.mode != 0) {
-            const any_u32x2 b = *reinterpret_cast<const any_u32x2 *>(g.data + at.ch);
+            const any_u32x2 b = global_at<any_u32x2>(g.data + at.ch);
             base = make_uint2(b.x, b.y);
         }
         base_words(base, bp);
@@ -916,10 +923,10 @@ __device__ __forceinline__ void coded_patch(const PrefixSeg &s, const PrefixSeg 
                                             uint16_t *lds) {
     const int tid = int(threadIdx.x);
     if (tid < s.n_esc) patch_one<R>(s, dim, t.rec, lds);
-    for (int i = tid + 64 * NW; i < s.n_esc; i += 64 * NW) patch_one<R>(s, dim, s.esc[i], lds);
+    for (int i = tid + 64 * NW; i < s.n_esc; i += 64 * NW) patch_one<R>(s, dim, global_at<uint32_t>(s.esc + i), lds);
     for (int k = 0; k < s.n_more; ++k) {
         const PrefixSeg g = seg_at(segs, s.more + k);
-        for (int i = tid; i < g.n_esc; i += 64 * NW) patch_one<R>(g, dim, g.esc[i], lds);
+        for (int i = tid; i < g.n_esc; i += 64 * NW) patch_one<R>(g, dim, global_at<uint32_t>(g.esc + i), lds);
     }
 }
 

@@ -40,5 +40,20 @@ __device__ __forceinline__ int seq_of(const BatchDev &b, int t) {
     return lo;
 }
 
+// The same by a whole wave, for a t that its lanes share: 64 starts at a time.
+__device__ __forceinline__ int seq_of_wave(const BatchDev &b, int t) {
+    if (b.starts == nullptr) return t / b.n_new;
+    if (t < b.starts[0] || t >= b.starts[b.n_seqs]) return -1;
+    int lo = 0, hi = b.n_seqs;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + kWave - 1) / kWave;
+        const int64_t at = int64_t(lo) + int64_t(lane_id()) * step;
+        const uint64_t below = __ballot(at < hi && b.starts[at] <= t);
+        lo += max(__popcll(below) - 1, 0) * step;
+        hi = min(lo + step, hi);
+    }
+    return lo;
+}
+
 } // namespace paged
 } // namespace kvexp_dev

@@ -98,26 +98,26 @@ __global__ __launch_bounds__(256) void prefix_segs_kernel(PrefixSeg *__restrict_
 }
 
 template <bool HALF, int W>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a, int rows_per_seq) {
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
     __shared__ float part[4][kMaxDim + 2];
     const int hq_all = a.n_kv * a.group;
     const int wave = int(threadIdx.x) >> 6, lane = lane_id();
     const int64_t at = W == 4 ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * 4 + wave;
-    const int seq = int(at / rows_per_seq);
-    if (seq >= a.batch.n_seqs) return;
-    const int rest = int(at - int64_t(seq) * rows_per_seq);
-    const int i = rest / hq_all, hq = rest - i * hq_all;
+    if (at >= int64_t(a.batch.n_tokens) * hq_all) return;
+    const int tok = int(at / hq_all), hq = int(at - int64_t(tok) * hq_all);
+    const int seq = seq_of_wave(a.batch, tok);
+    if (seq < 0) return; // a row behind the last sequence
     Rows r;
     find_rows(a, seq, 1, 1, 1, r); // (split and tile 1: no errors raised here)
-    if (i >= r.n) return;
+    const int i = tok - r.first;
+    if (i < 0 || i >= r.n) return;
     const int head = hq / a.group, g = hq - head * a.group;
-    const int64_t tok = r.first + i;
     const int first = W == 4 ? wave : 0;
     Joined j;
     if (a.s_splits > 0) {
         const int len = split_tokens(a.s_len, a.s_splits, a.s_min_split);
         const int n = max(1, (a.s_len + len - 1) / len);
-        join(j, a.s_acc, a.s_ml, int64_t(head) * a.s_splits * a.s_rows + tok * a.group + g, a.s_rows, first, W, n, a.dim);
+        join(j, a.s_acc, a.s_ml, int64_t(head) * a.s_splits * a.s_rows + int64_t(tok) * a.group + g, a.s_rows, first, W, n, a.dim);
     }
     const int n = max(1, (r.len + r.split_len - 1) / r.split_len);
     join(j, a.acc, a.ml, state_slot(a, r, head, 0, i * a.group + g), a.max_rows, first, W, n, a.dim);
@@ -147,9 +147,9 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a, int r
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int d = lane + kWave * k;
-        if (d < a.dim) a.out.p[tok * a.out.token + int64_t(hq) * a.out.head + d] = to_16<HALF>(finish(j.acc[k], j.l));
+        if (d < a.dim) a.out.p[int64_t(tok) * a.out.token + int64_t(hq) * a.out.head + d] = to_16<HALF>(finish(j.acc[k], j.l));
     }
-    if (lane == 0 && a.lse != nullptr) a.lse[tok * hq_all + hq] = log_sum(j.m, j.l);
+    if (lane == 0 && a.lse != nullptr) a.lse[at] = log_sum(j.m, j.l);
 }
 
 } // namespace
@@ -190,13 +190,12 @@ hipError_t prefix_segs(PrefixSeg *segs, int n, const EscJob *jobs, hipStream_t s
 }
 
 hipError_t paged_merge(const PagedAttnArgs &a, bool half, hipStream_t s) {
-    const int rows = a.batch.max_new * a.n_kv * a.group;
-    const int64_t n = int64_t(a.batch.n_seqs) * rows;
+    const int64_t n = int64_t(a.batch.n_tokens) * a.n_kv * a.group;
     // four waves per row where the rows alone do not fill the GPU and there
     // are splits for them
     const bool four = n < 4096 && a.n_splits + a.s_splits >= 8;
     auto run = [&](auto kernel, int64_t groups) {
-        hipLaunchKernelGGL(kernel, dim3(unsigned(groups)), dim3(256), 0, s, a, rows);
+        hipLaunchKernelGGL(kernel, dim3(unsigned(groups)), dim3(256), 0, s, a);
     };
     if (four) half ? run(paged::paged_merge_kernel<true, 4>, n) : run(paged::paged_merge_kernel<false, 4>, n);
     else half ? run(paged::paged_merge_kernel<true, 1>, (n + 3) / 4) : run(paged::paged_merge_kernel<false, 1>, (n + 3) / 4);

@@ -95,7 +95,7 @@ struct PrefixTensor {
 
 // The attention calls. Partial states: slot (row, split) holds m, l (in the
 // base-2 exponent's units) and dim sums; `acc` row-major [slot][dim], `ml`
-// [slot][2].
+// [slot][2]; slots [head][split][token row, query head of the group].
 struct PagedAttnArgs {
     PoolDev pool;
     BatchDev batch;
@@ -110,7 +110,7 @@ struct PagedAttnArgs {
     int32_t row_tiles;
     int32_t shared;   // rows of all sequences against one table of `len` tokens
     int32_t len;
-    int32_t max_rows; // rows of a (sequence, head): slot stride
+    int32_t max_rows; // query rows of a KV head in the call: slot stride
     float *acc, *ml;
     uint32_t *status;
     const PrefixTensor *px; // [2 n_kv] (K, V of each head), shared prefixes kept as containers

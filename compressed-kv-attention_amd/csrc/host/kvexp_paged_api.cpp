@@ -4,11 +4,9 @@
 #include "api_common.hpp"
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
-#ifndef XROWS
-#define XROWS 128
-#endif
 #include <cstring>
 
 #include "../hip/paged_types.h"
@@ -33,7 +31,10 @@ struct kvexp_hip_prefix {
 namespace {
 
 constexpr int kMaxHeadDim = 256;
-constexpr int64_t kGridMax = (int64_t(1) << 24) - 1; // workgroups of 256 threads below 2^32 threads
+constexpr int64_t kThreadsMax = int64_t(UINT32_MAX);  // of a launch
+constexpr int64_t kTokensMax = int64_t(1) << 30;       // of a sequence: a tile's end stays an int
+constexpr int64_t kRotTokensMax = int64_t(1) << 27;    // new tokens of a rotation: its threads stay a launch's
+constexpr int64_t kRotChannelsMax = int64_t(1) << 26;  // a token's channels over all heads: 16 tokens' stay an int
 
 [[noreturn]] void bad(const std::string &msg) { fail(KVEXP_HIP_INVALID_ARGUMENT, msg); }
 
@@ -109,7 +110,7 @@ BatchDev batch_of(const char *who, const kvexp_hip_batch *b, int page_tokens, in
     if (b->lens == nullptr || (b->table == nullptr && b->table_width > 0)) bad(std::string(who) + ": null table or lens");
     if (b->n_seqs > 1 && b->table_stride < b->table_width) bad(std::string(who) + ": rows of the page table overlap");
     const int64_t most = int64_t(b->table_width) * page_tokens;
-    if (most > INT32_MAX) fail(KVEXP_HIP_UNSUPPORTED, std::string(who) + ": a page table of 2^31 tokens or more");
+    if (most > kTokensMax) fail(KVEXP_HIP_UNSUPPORTED, std::string(who) + ": a page table of more than 2^30 tokens");
     if (b->starts == nullptr) {
         if (b->n_tokens % b->n_seqs != 0)
             bad(std::string(who) + ": without starts every sequence has n_tokens / n_seqs new tokens");
@@ -149,9 +150,14 @@ RopeDev rope_of(const char *who, const kvexp_hip_rope *r, const kvexp_hip_positi
     return d;
 }
 
+void check_rotation(const char *who, int n_tokens, int64_t channels) {
+    if (n_tokens > kRotTokensMax || channels > kRotChannelsMax)
+        fail(KVEXP_HIP_UNSUPPORTED, std::string(who) + ": more tokens or heads than a launch takes");
+}
+
 // How a call is cut.
 struct Cut {
-    int tile_rows = 16, row_tiles = 1, n_splits = 1, min_split = 64, rows = 0;
+    int tile_rows = 16, row_tiles = 1, n_splits = 1, min_split = 64;
 };
 
 // Rows per (sequence, head) pick the kernel: what a workgroup of the few-row
@@ -159,9 +165,8 @@ struct Cut {
 Cut cut_of(const kvexp_hip_ctx *ctx, int64_t rows, int64_t pairs, int max_len, int dim, bool coded) {
     Cut c;
     if (rows > INT32_MAX / 2) fail(KVEXP_HIP_UNSUPPORTED, "paged attention: too many query rows");
-    c.rows = int(rows);
     const bool many = coded || rows > few_rows(dim);
-    c.tile_rows = !many ? (rows > 16 ? 32 : 16) : rows > XROWS ? many_rows(dim, coded) : 128;
+    c.tile_rows = !many ? (rows > 16 ? 32 : 16) : rows > 128 ? many_rows(dim, coded) : 128;
     c.row_tiles = int((rows + c.tile_rows - 1) / c.tile_rows);
     c.min_split = 256;
     const int64_t target = int64_t(std::max(1, ctx->cu_count)) * (many ? (c.tile_rows == 256 ? 1 : 2) : 8);
@@ -174,6 +179,14 @@ Cut cut_of(const kvexp_hip_ctx *ctx, int64_t rows, int64_t pairs, int max_len, i
     const int64_t even = (int64_t(max_len) + c.n_splits - 1) / c.n_splits;
     c.min_split = int(std::max<int64_t>(c.min_split, (even + 63) / 64 * 64));
     return c;
+}
+
+// Threads of the launch over `pairs` (sequence, head) pairs.
+int64_t threads_of(const Cut &c, int64_t pairs) {
+    if (pairs > kThreadsMax) return INT64_MAX;
+    const int64_t per = int64_t(c.row_tiles) * c.n_splits; // < 2^31 * 2^8
+    const int64_t threads = c.tile_rows == 256 ? 512 : 256;
+    return per > kThreadsMax / threads / std::max<int64_t>(1, pairs) ? INT64_MAX : per * pairs * threads;
 }
 
 struct Call {
@@ -211,6 +224,8 @@ Call plan_call(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, const kvexp_hip
             if (shared->n_tokens != p.seq) bad(std::string(who) + ": n_tokens must be the prefix's");
         } else {
             if (shared->n_tokens <= 0) bad(std::string(who) + ": an empty shared prefix");
+            if (shared->n_tokens > kTokensMax)
+                fail(KVEXP_HIP_UNSUPPORTED, std::string(who) + ": a shared prefix of more than 2^30 tokens");
             if (int64_t(shared->table_width) * pages->page_tokens < shared->n_tokens)
                 bad(std::string(who) + ": the shared prefix's table is shorter than its tokens");
         }
@@ -221,16 +236,17 @@ Call plan_call(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, const kvexp_hip
         bad(std::string(who) + ": the prefix is on another device");
     const int64_t rows = int64_t(a.batch.max_new) * a.group;
     c.cut = cut_of(ctx, rows, int64_t(a.batch.n_seqs) * a.n_kv, max_len, a.dim, false);
-    if (int64_t(a.batch.n_seqs) * a.n_kv * c.cut.row_tiles * c.cut.n_splits > kGridMax ||
-        int64_t(a.batch.n_seqs) * a.batch.max_new * n_q_heads > INT32_MAX)
+    // (the merge: a wave per query row)
+    if (threads_of(c.cut, int64_t(a.batch.n_seqs) * a.n_kv) > kThreadsMax ||
+        int64_t(a.batch.n_tokens) * n_q_heads > kThreadsMax / 64 - 4)
         fail(KVEXP_HIP_UNSUPPORTED, std::string(who) + ": more sequences or query rows than a launch takes");
     a.row_tiles = c.cut.row_tiles;
     a.n_splits = c.cut.n_splits;
     a.min_split = c.cut.min_split;
-    a.max_rows = c.cut.rows;
+    a.max_rows = a.batch.n_tokens * a.group;
     a.direct = !c.has_shared && a.n_splits == 1;
     if (!a.direct) {
-        c.slots = int64_t(a.batch.n_seqs) * a.n_kv * a.n_splits * a.max_rows;
+        c.slots = int64_t(a.n_kv) * a.n_splits * a.max_rows;
         c.at_ml = padded(size_t(c.slots) * size_t(a.dim) * sizeof(float));
         c.bytes = c.at_ml + padded(size_t(c.slots) * 2 * sizeof(float));
     }
@@ -242,12 +258,11 @@ Call plan_call(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, const kvexp_hip
         p.len = shared->n_tokens;
         const bool xkv = shared->xkv != nullptr;
         c.shared_cut = cut_of(ctx, int64_t(a.batch.n_tokens) * a.group, a.n_kv, p.len, a.dim, xkv);
-        if (int64_t(a.n_kv) * c.shared_cut.row_tiles * c.shared_cut.n_splits > kGridMax)
+        if (threads_of(c.shared_cut, a.n_kv) > kThreadsMax)
             fail(KVEXP_HIP_UNSUPPORTED, std::string(who) + ": more query rows than a launch takes");
         p.row_tiles = c.shared_cut.row_tiles;
         p.n_splits = c.shared_cut.n_splits;
         p.min_split = c.shared_cut.min_split;
-        p.max_rows = c.shared_cut.rows;
         if (xkv) p.px = shared->xkv->tensors;
         else {
             p.batch.table = shared->table;
@@ -404,6 +419,7 @@ int kvexp_hip_rope_rows(kvexp_hip_ctx *ctx, const kvexp_hip_rope *rope, const kv
         if (n_tokens < 0 || n_heads <= 0) bad(std::string(who) + ": empty rows");
         RotateArgs a{};
         a.rope = rope_of(who, rope, positions, dim, n_tokens);
+        check_rotation(who, n_tokens, int64_t(n_heads) * dim);
         if (n_tokens == 0) return;
         check_rows(who, "x", x);
         check_rows(who, "out", out);
@@ -433,6 +449,7 @@ int kvexp_hip_paged_append(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, con
         if ((q == nullptr) != (q_out == nullptr)) bad(std::string(who) + ": q and q_out go together");
         if (q != nullptr && rope == nullptr) bad(std::string(who) + ": queries without a rotation");
         if (q != nullptr && n_q_heads <= 0) bad(std::string(who) + ": no query heads");
+        check_rotation(who, a.batch.n_tokens, (int64_t(q != nullptr ? n_q_heads : 0) + 2 * int64_t(pages->n_heads)) * pages->dim);
         if (d_status == nullptr) bad(std::string(who) + ": null status word");
         if (a.batch.n_tokens == 0) return;
         check_rows(who, "k", k);
@@ -466,6 +483,7 @@ int kvexp_hip_prefix_create(kvexp_hip_ctx *ctx, const kvexp_hip_head *heads, int
         check_dim(who, dim);
         const int seq = heads[0].seq;
         if (seq <= 0) bad(std::string(who) + ": an empty shared prefix");
+        if (seq > kTokensMax) fail(KVEXP_HIP_UNSUPPORTED, std::string(who) + ": a shared prefix of more than 2^30 tokens");
         for (int h = 0; h < n_heads; ++h) {
             const kvexp_hip_head &H = heads[h];
             if (H.k_xkv == nullptr || H.v_xkv == nullptr || H.k_offsets == nullptr || H.v_offsets == nullptr ||
@@ -524,7 +542,12 @@ int kvexp_hip_paged_attention(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, 
             bad(std::string(who) + ": the workspace must be 16-byte aligned");
         if (workspace_bytes < c.bytes)
             fail(KVEXP_HIP_CAPACITY, std::string(who) + ": workspace below kvexp_hip_paged_attention_workspace");
-        const float scale2 = float(double(scale) * 1.4426950408889634074);
+        // never 0, which times a masked place's -inf is no number: the least
+        // normal number instead (with products q . k up to 2^100 the weights
+        // are those of scale 0 to 2^-26)
+        float scale2 = float(double(scale) * 1.4426950408889634074);
+        if (!std::isfinite(scale2)) bad(std::string(who) + ": the scale is past float's range");
+        if (std::fabs(scale2) < FLT_MIN) scale2 = std::copysign(FLT_MIN, scale2);
         auto *w = static_cast<uint8_t *>(workspace);
         PagedAttnArgs &a = c.own;
         a.q = rows_in(q);

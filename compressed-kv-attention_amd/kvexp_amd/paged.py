@@ -19,8 +19,6 @@ from __future__ import annotations
 import ctypes as C
 import math
 
-DTYPES = ("bfloat16", "float16")
-
 
 class _Pages(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p),
@@ -69,61 +67,103 @@ def declare(L, head) -> None:
     L.kvexp_hip_paged_status.argtypes = [vp, vp, vp]
 
 
+_torch = _lib = None
+
+
+def _load():
+    """torch and the library, once (importing this module loads neither)."""
+    global _torch, _lib
+    if _lib is None:
+        import torch
+
+        import kvexp_amd
+
+        _torch, _lib = torch, kvexp_amd.lib()
+    return _torch, _lib
+
+
 def _kv():
     import kvexp_amd
 
     return kvexp_amd
 
 
+def _check(rc: int) -> None:
+    if rc:
+        _kv().check(rc)
+
+
 def _dtype_code(who: str, dtype) -> int:
-    name = str(dtype).replace("torch.", "")
-    if name not in DTYPES:
-        raise ValueError(f"{who}: elements are bfloat16 or float16, not {name}")
-    return DTYPES.index(name)
+    torch = _torch_module()
+    if dtype is torch.bfloat16:
+        return 0
+    if dtype is torch.float16:
+        return 1
+    raise ValueError(f"{who}: elements are bfloat16 or float16, not {dtype}")
+
+
+def _torch_module():
+    if _torch is not None:
+        return _torch
+    import torch
+
+    return torch
 
 
 def _check_rows(who: str, name: str, t, dtype, n=None, heads=None, dim=None) -> None:
-    if t.dim() != 3:
+    shape = t.shape
+    if len(shape) != 3:
         raise ValueError(f"{who}: {name} must be [tokens, heads, head_dim]")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{who}: {name} must be {dtype}, not {t.dtype}")
-    want = (n, heads, dim)
-    if any(w is not None and int(s) != w for s, w in zip(t.shape, want)):
-        raise ValueError(f"{who}: {name} must be {list(want)}, not {list(t.shape)}")
+    if (n is not None and shape[0] != n) or (heads is not None and shape[1] != heads) or \
+            (dim is not None and shape[2] != dim):
+        raise ValueError(f"{who}: {name} must be {[n, heads, dim]}, not {list(shape)}")
 
 
 def _check_device(who: str, device: int, **tensors) -> None:
     for name, t in tensors.items():
-        if t is not None and (t.device.type != "cuda" or t.device.index != device):
+        if t is not None and t.get_device() != device:  # (-1: not on a GPU)
             raise ValueError(f"{who}: {name} must be on cuda:{device}, not {t.device}")
 
 
-def _fits(t) -> bool:
-    return (t.stride(2) == 1 or t.shape[2] == 1) and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 \
-        and t.data_ptr() % 16 == 0
-
-
-def _rows(t) -> _Rows:
-    return _Rows(t.data_ptr(), t.stride(0), t.stride(1))
+def _rows(t) -> _Rows | None:
+    """t as the kernels read it; None where its layout is not one they do."""
+    token, head, channel = t.stride()
+    p = t.data_ptr()
+    if (channel != 1 and t.shape[2] != 1) or (token | head) % 8 or p % 16:
+        return None
+    return _Rows(p, token, head)
 
 
 def _readable(t):
-    """t, or a copy of it where its layout is not one the kernels read."""
-    import torch
+    """(rows, what they point at): t, or a copy of it where its layout is not one the kernels read."""
+    r = _rows(t)
+    if r is None:
+        t = t.clone(memory_format=_torch_module().contiguous_format)
+        r = _rows(t)
+    return r, t
 
-    return t if t.numel() == 0 or _fits(t) else t.clone(memory_format=torch.contiguous_format)
+
+def _writable(who: str, name: str, t) -> _Rows:
+    r = _rows(t)
+    if r is None:
+        raise ValueError(f"{who}: {name} must have contiguous channels, strides of multiples of 8 and 16-byte alignment")
+    if (r.token == 0 and t.shape[0] > 1) or (r.head == 0 and t.shape[1] > 1):
+        raise ValueError(f"{who}: rows of {name} lie on one another")
+    return r
 
 
 class _on:
-    """torch's current stream set to `stream` for the allocations inside (None: as it is)."""
+    """torch's current stream set to `stream` for what is inside (None: as it is)."""
 
     def __init__(self, stream):
-        import torch
-
-        if stream is not None and not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(int(stream))
-        self.stream = stream
-        self.guard = None if stream is None else torch.cuda.stream(stream)
+        self.guard = None
+        if stream is not None:
+            torch = _torch_module()
+            if not isinstance(stream, torch.cuda.Stream):
+                stream = torch.cuda.ExternalStream(int(stream))
+            self.guard = torch.cuda.stream(stream)
 
     def __enter__(self):
         if self.guard is not None:
@@ -134,10 +174,8 @@ class _on:
             self.guard.__exit__(*e)
 
 
-def _raw_stream(device: int):
-    import torch
-
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _raw_stream(device: int) -> int:
+    return _torch_module()._C._cuda_getCurrentRawStream(device)
 
 
 class Rope:
@@ -150,9 +188,10 @@ class Rope:
     """
 
     def __init__(self, inv_freq, axes=None, interleaved: bool = False, scale: float = 1.0):
-        if inv_freq.dim() != 1 or str(inv_freq.dtype) != "torch.float32" or inv_freq.numel() == 0:
+        torch = _torch_module()
+        if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float32 or inv_freq.numel() == 0:
             raise ValueError("kvexp.Rope: inv_freq must be float32 [n]")
-        if axes is not None and (str(axes.dtype) != "torch.uint8" or axes.shape != inv_freq.shape):
+        if axes is not None and (axes.dtype is not torch.uint8 or axes.shape != inv_freq.shape):
             raise ValueError("kvexp.Rope: axes must be uint8, one per frequency")
         if not math.isfinite(scale):
             raise ValueError("kvexp.Rope: the scale is not finite")
@@ -172,45 +211,44 @@ def _positions(who: str, device: int, positions, offset: int, n: int):
     """(_Positions, axes, what it points at)."""
     if positions is None:
         return _Positions(None, 0, int(offset), 0, 0), 1, None
-    if positions.dim() == 1:
-        positions = positions[None]
-    if positions.dim() != 2 or positions.shape[1] != n or positions.shape[0] == 0:
+    torch = _torch_module()
+    shape = positions.shape
+    if len(shape) not in (1, 2) or shape[-1] != n or shape[0] == 0:
         raise ValueError(f"{who}: positions must be [tokens] or [axes, tokens] with {n} tokens")
-    wide = str(positions.dtype) == "torch.int64"
-    if not wide and str(positions.dtype) != "torch.int32":
+    wide = positions.dtype is torch.int64
+    if not wide and positions.dtype is not torch.int32:
         raise ValueError(f"{who}: positions must be int32 or int64")
     _check_device(who, device, positions=positions)
-    if positions.stride(1) != 1 or (positions.shape[0] > 1 and positions.stride(0) < n):
+    axes = 1 if len(shape) == 1 else int(shape[0])
+    if positions.stride(-1) != 1 or (axes > 1 and positions.stride(0) < n):
         positions = positions.contiguous()
-    return (_Positions(positions.data_ptr(), positions.stride(0), 0, int(wide), 0), int(positions.shape[0]),
-            positions)
+    return _Positions(positions.data_ptr(), positions.stride(0) if axes > 1 else 0, 0, int(wide), 0), axes, positions
 
 
 def rope(ctx, x, positions, rope: Rope, out=None, inverse: bool = False, stream=None):
     """x [tokens, heads, head_dim] rotated by `rope` at `positions` ([tokens], [axes, tokens], or None for 0, 1, 2, ..),
     into out (which may be x) or a new tensor; inverse: rotated back."""
-    import torch
-
-    kv, who = _kv(), "kvexp.rope"
+    who = "kvexp.rope"
     code = _dtype_code(who, x.dtype)
     _check_rows(who, "x", x, x.dtype)
-    n, heads, dim = (int(s) for s in x.shape)
+    n, heads, dim = x.shape
+    if dim == 0 or dim % 8 or dim > 256:
+        raise ValueError(f"{who}: head_dim must be a multiple of 8 and at most 256")
     if out is not None:
         _check_rows(who, "out", out, x.dtype, n, heads, dim)
-        if not _fits(out):
-            raise ValueError(f"{who}: out must have contiguous channels, strides of multiples of 8, 16-byte alignment")
     _check_device(who, ctx.device, x=x, out=out)
-    with _on(stream):
-        x = x.detach()
-        at, axes, keep = _positions(who, ctx.device, positions, 0, n)
-        r = rope._struct(who, ctx.device, dim, axes)
-        src = _readable(x)
-        if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if x.numel():
-            kv.check(kv.lib().kvexp_hip_rope_rows(ctx.h, r, at, _rows(src), _rows(out), n, heads, dim, code,
-                                                  int(inverse), _raw_stream(ctx.device)))
-    del keep
+    if stream is not None:
+        with _on(stream):
+            return globals()["rope"](ctx, x, positions, rope, out, inverse)
+    torch, L = _load()
+    at, axes, keep = _positions(who, ctx.device, positions, 0, n)
+    r = rope._struct(who, ctx.device, dim, axes)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    to = _writable(who, "out", out)
+    if n and heads:
+        src, x = _readable(x)
+        _check(L.kvexp_hip_rope_rows(ctx.h, r, at, src, to, n, heads, dim, code, int(inverse), _raw_stream(ctx.device)))
     return out
 
 
@@ -226,12 +264,12 @@ class Batch:
     """
 
     def __init__(self, table, lens, starts=None, max_new: int | None = None, max_len: int | None = None):
-        who = "kvexp.Batch"
+        who, i32 = "kvexp.Batch", _torch_module().int32
         for name, t, d in (("table", table, 2), ("lens", lens, 1), ("starts", starts, 1)):
-            if t is not None and (t.dim() != d or str(t.dtype) != "torch.int32"):
+            if t is not None and (t.dim() != d or t.dtype is not i32):
                 raise ValueError(f"{who}: {name} must be int32 with {d} dimension{'s' if d > 1 else ''}")
         n = int(lens.shape[0])
-        if int(table.shape[0]) != n or (starts is not None and int(starts.shape[0]) != n + 1):
+        if table.shape[0] != n or (starts is not None and starts.shape[0] != n + 1):
             raise ValueError(f"{who}: table and lens have one row per sequence, starts one more")
         self.table = table if table.stride(1) == 1 or table.shape[1] <= 1 else table.contiguous()
         self.lens, self.starts = lens.contiguous(), None if starts is None else starts.contiguous()
@@ -289,7 +327,7 @@ class PagePrefix:
 
     def __init__(self, cache, table, seq: int):
         who = "kvexp.PagePrefix"
-        if table.dim() != 1 or str(table.dtype) != "torch.int32":
+        if table.dim() != 1 or table.dtype is not _torch_module().int32:
             raise ValueError(f"{who}: table must be int32 [pages]")
         if seq <= 0 or int(table.shape[0]) * cache.page_tokens < seq:
             raise ValueError(f"{who}: {int(seq)} tokens in {int(table.shape[0])} pages of {cache.page_tokens}")
@@ -334,6 +372,7 @@ class PagedCache:
         self.k = torch.empty(shape, dtype=dtype, device=dev) if k is None else k
         self.v = torch.empty(shape, dtype=dtype, device=dev) if v is None else v
         self.status_word = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._sizes = {}
         sk, sv = self.k.stride(), self.v.stride()
         self._struct = _Pages(self.k.data_ptr(), self.v.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
                               self._code, shape[0], shape[2], shape[1], shape[3], 0)
@@ -347,10 +386,8 @@ class PagedCache:
         """Writes the batch's new keys (rotated by `rope`) and values [tokens, n_heads, head_dim] to their pages;
         returns q [tokens, query heads, head_dim] rotated (into q_out, which may be q), or None. positions: [tokens] or
         [axes, tokens]; None: each token's index in its sequence plus `offset` (the tokens of a shared prefix)."""
-        import torch
-
-        kv, who = _kv(), "kvexp.paged_append"
-        n = int(k.shape[0])
+        who = "kvexp.paged_append"
+        n = int(k.shape[0]) if k.dim() else 0
         _check_rows(who, "k", k, self.dtype, n, self.n_heads, self.dim)
         _check_rows(who, "v", v, self.dtype, n, self.n_heads, self.dim)
         if q is not None:
@@ -361,25 +398,26 @@ class PagedCache:
             if q is None:
                 raise ValueError(f"{who}: q and q_out go together")
             _check_rows(who, "q_out", q_out, self.dtype, *q.shape)
-            if not _fits(q_out):
-                raise ValueError(f"{who}: q_out must have contiguous channels, strides of multiples of 8, 16-byte "
-                                 "alignment")
         _check_device(who, self.ctx.device, k=k, v=v, q=q, q_out=q_out)
-        with _on(stream):
-            at, axes, keep = _positions(who, self.ctx.device, positions, offset, n)
-            r = None if rope is None else rope._struct(who, self.ctx.device, self.dim, axes)
-            b = batch._struct(who, self.ctx.device, n)
-            if q is not None and q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            if n and (q is None or q.shape[1]):
-                k, v, src = _readable(k), _readable(v), None if q is None else _readable(q)
-                kv.check(kv.lib().kvexp_hip_paged_append(
-                    self.ctx.h, self._struct, b, _rows(k), _rows(v), r, at, None if src is None else _rows(src),
-                    None if src is None else _rows(q_out), 0 if src is None else int(src.shape[1]),
-                    self.status_word.data_ptr(), _raw_stream(self.ctx.device)))
-            if check_errors:
-                self.status()
-        del keep
+        if stream is not None:
+            with _on(stream):
+                return self.append(k, v, batch, rope, positions, offset, q, q_out, check_errors)
+        torch, L = _load()
+        at, axes, keep = _positions(who, self.ctx.device, positions, offset, n)
+        r = None if rope is None else rope._struct(who, self.ctx.device, self.dim, axes)
+        b = batch._struct(who, self.ctx.device, n)
+        if q is not None and q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        to = None if q is None else _writable(who, "q_out", q_out)
+        if n:
+            (kr, k), (vr, v) = _readable(k), _readable(v)
+            qr, heads = None, 0
+            if q is not None and q.shape[1]:
+                (qr, q), heads = _readable(q), int(q.shape[1])
+            _check(L.kvexp_hip_paged_append(self.ctx.h, self._struct, b, kr, vr, r, at, qr, to if heads else None, heads,
+                                            self.status_word.data_ptr(), _raw_stream(self.ctx.device)))
+        if check_errors:
+            self.status()
         return q_out
 
     def attention(self, q, batch: Batch, scale: float | None = None, prefix=None, out=None, lse=None,
@@ -388,45 +426,50 @@ class PagedCache:
         or PagePrefix that every sequence shares): token i of a sequence's n new ones sees the first len - n + i + 1
         tokens of it. scale: of the scores (None: 1 / sqrt(head_dim)). Returns out, or (out, lse [tokens, query
         heads] float32) with return_lse; a token that sees nothing gives 0 and -inf."""
-        import torch
-
-        kv, who = _kv(), "kvexp.paged_attention"
+        who = "kvexp.paged_attention"
         _check_rows(who, "q", q, self.dtype, None, None, self.dim)
-        n, heads = int(q.shape[0]), int(q.shape[1])
+        n, heads, _ = q.shape
         if heads == 0 or heads % self.n_heads:
             raise ValueError(f"{who}: {heads} query heads over {self.n_heads} heads")
         if out is not None:
             _check_rows(who, "out", out, self.dtype, n, heads, self.dim)
-            if not _fits(out):
-                raise ValueError(f"{who}: out must have contiguous channels, strides of multiples of 8, 16-byte "
-                                 "alignment")
-        if lse is not None and (tuple(lse.shape) != (n, heads) or lse.dtype != torch.float32
+        if lse is not None and (tuple(lse.shape) != (n, heads) or lse.dtype is not _torch_module().float32
                                 or not lse.is_contiguous()):
             raise ValueError(f"{who}: lse must be contiguous float32 [{n}, {heads}]")
         scale = 1.0 / math.sqrt(self.dim) if scale is None else float(scale)
         if not math.isfinite(scale):
             raise ValueError(f"{who}: the scale is not finite")
         _check_device(who, self.ctx.device, q=q, out=out, lse=lse)
-        with _on(stream):
-            b = batch._struct(who, self.ctx.device, n)
-            sh = None if prefix is None else prefix._struct(who, self)
-            src = _readable(q.detach())
-            if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            if lse is None and return_lse:
-                lse = torch.empty((n, heads), dtype=torch.float32, device=q.device)
-            L = kv.lib()
+        if stream is not None:
+            with _on(stream):
+                return self.attention(q, batch, scale, prefix, out, lse, return_lse, check_errors)
+        torch, L = _load()
+        b = batch._struct(who, self.ctx.device, n)
+        sh = None if prefix is None else prefix._struct(who, self)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        to = _writable(who, "out", out)
+        if lse is None and return_lse:
+            lse = torch.empty((n, heads), dtype=torch.float32, device=q.device)
+        # the workspace follows the sizes of the call
+        key = (n, heads, b.n_seqs, b.table_width, b.starts is None, b.max_new, b.max_len,
+               None if sh is None else (sh.xkv is None, sh.n_tokens))
+        size = self._sizes.get(key)
+        if size is None:
             size = L.kvexp_hip_paged_attention_workspace(self.ctx.h, self._struct, b, sh, heads)
             if size < 0:
-                raise kv.KvexpHipError(1, L.kvexp_hip_last_error().decode())
+                raise _kv().KvexpHipError(1, L.kvexp_hip_last_error().decode())
+            if len(self._sizes) >= 1024:
+                self._sizes.clear()
+            self._sizes[key] = size
+        if n:
             ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-            if n:
-                kv.check(L.kvexp_hip_paged_attention(
-                    self.ctx.h, self._struct, b, sh, _rows(src), heads, scale, _rows(out),
-                    None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), size,
-                    self.status_word.data_ptr(), _raw_stream(self.ctx.device)))
-            if check_errors:
-                self.status()
+            src, q = _readable(q)
+            _check(L.kvexp_hip_paged_attention(
+                self.ctx.h, self._struct, b, sh, src, heads, scale, to, None if lse is None else lse.data_ptr(),
+                None if ws is None else ws.data_ptr(), size, self.status_word.data_ptr(), _raw_stream(self.ctx.device)))
+        if check_errors:
+            self.status()
         return (out, lse) if return_lse else out
 
     def status(self, stream=None) -> None:

@@ -336,3 +336,97 @@ def test_rows_behind_the_last_sequence(ctx):
     cache.attention(q, kv.Batch(c["table"], c["lens"], c["starts"]), out=out, check_errors=True)
     assert bool((out[3:] == 9).all())
     ref.check_attention(out[:3], None, ref.batch_reference(c, lens, new, q[:3], 1 / 8), BF, False)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.2, 1e-30, 1e-44])
+@pytest.mark.parametrize("new,group,dim", [(1, 4, 64), (5, 4, 64), (20, 4, 64), (70, 4, 128), (9, 4, 256)])
+def test_scales(ctx, scale, new, group, dim):
+    """Scales of 0, below float's normal numbers and below 0, over masked places."""
+    import kvexp_amd as kv
+
+    g = gen(new + dim)
+    lens, page = [77, 300], 16
+    c = ref.make_batch(g, lens, [new] * 2, page, 1, dim, BF)
+    q = torch.randn(2 * new, group, dim, generator=g).to(BF).cuda()
+    cache = kv.PagedCache(ctx, 1, dim, c["k"].shape[0], page, BF, k=c["k"], v=c["v"])
+    say("scale", scale, new, group, dim)
+    out, lse = cache.attention(q, kv.Batch(c["table"], c["lens"]), scale, return_lse=True, check_errors=True)
+    ref.check_attention(out, lse, ref.batch_reference(c, lens, [new] * 2, q, scale), BF, split_p=new * group <= 16)
+
+
+@pytest.mark.parametrize("seqs", [64, 65, 130, 300])
+def test_many_ragged_sequences(ctx, seqs):
+    """Counts of sequences about the merge's 64 starts at a time, some without new tokens, over several splits."""
+    import kvexp_amd as kv
+
+    g = gen(seqs)
+    new = torch.randint(0, 3, (seqs,), generator=g).tolist()
+    lens = [(37 * b) % 90 + n for b, n in enumerate(new)]
+    lens[seqs // 2] = 2500
+    new[seqs // 2] = 2
+    page, dim = 64, 32
+    c = ref.make_batch(g, lens, new, page, 1, dim, BF)
+    q = torch.randn(sum(new) + 3, 2, dim, generator=g).to(BF).cuda()
+    cache = kv.PagedCache(ctx, 1, dim, c["k"].shape[0], page, BF, k=c["k"], v=c["v"])
+    want = ref.batch_reference(c, lens, new, q[:-3], 0.3)
+    for max_new in (2, None):
+        out = torch.full_like(q, 9.0)
+        say("ragged", seqs, max_new)
+        cache.attention(q, kv.Batch(c["table"], c["lens"], c["starts"], max_new), 0.3, out=out, check_errors=True)
+        ref.check_attention(out[:-3], None, want, BF, False)
+        assert bool((out[-3:] == 9).all())
+
+
+def test_outputs_whose_rows_overlap_are_refused(ctx):
+    import kvexp_amd as kv
+
+    x = torch.randn(3, 4, 64).to(BF).cuda()
+    with pytest.raises(ValueError, match="on one another"):
+        ctx.rope(x, None, kv.Rope(freqs(32)), out=torch.zeros(1, 4, 64, dtype=BF, device="cuda").expand(3, 4, 64))
+    with pytest.raises(ValueError, match="on one another"):
+        ctx.rope(x, None, kv.Rope(freqs(32)), out=torch.zeros(3, 1, 64, dtype=BF, device="cuda").expand(3, 4, 64))
+
+
+def test_rope_traced_and_captured(ctx):
+    """Forward and gradient through a trace of both, twice differentiated, and captured into a graph and replayed."""
+    import kvexp_amd.torch_ops  # noqa: F401
+
+    g = gen(8)
+    x = torch.randn(33, 3, 64, generator=g).to(BF).cuda().requires_grad_()
+    dy = torch.randn(33, 3, 64, generator=g).to(BF).cuda().requires_grad_()
+    freq, pos = freqs(32), torch.randint(0, 5000, (33,), generator=g).cuda()
+
+    def both(x, dy):
+        y = torch.ops.kvexp.rope(x, pos, freq)
+        return y, torch.autograd.grad(y, x, dy, create_graph=True)[0]
+
+    y, dx = both(x, dy)
+    (ddy,) = torch.autograd.grad(dx, dy, x.detach())  # the gradient of the gradient's is the rotation
+    assert torch.equal(ddy, y.detach())
+    y, dx = y.detach(), dx.detach()
+    say("trace")
+    fn = torch.compile(lambda x: torch.ops.kvexp.rope(x, pos, freq) * 2, backend="aot_eager", fullgraph=True)
+    z = fn(x)
+    assert torch.equal(z, 2 * y)
+    assert torch.equal(torch.autograd.grad(z, x, dy.detach() / 2)[0], dx)
+
+    say("capture")
+    xs, ds = x.detach().clone().requires_grad_(), dy.detach().clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(torch.ops.kvexp.rope(xs, pos, freq), xs, ds)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = torch.ops.kvexp.rope(xs, pos, freq)
+        (grad,) = torch.autograd.grad(out, xs, ds)
+    for i in range(3):
+        with torch.no_grad():
+            xs.copy_(torch.randn(33, 3, 64, generator=g)), ds.copy_(torch.randn(33, 3, 64, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        e = xs.detach().clone().requires_grad_()
+        want = torch.ops.kvexp.rope(e, pos, freq)
+        assert torch.equal(out, want) and torch.equal(grad, torch.autograd.grad(want, e, ds)[0])
+        torch.cuda.synchronize()

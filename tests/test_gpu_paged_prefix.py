@@ -329,3 +329,20 @@ def test_no_float_is_read_past_the_pools(ctx):
         out, lse = cache.attention(q, batch, return_lse=True, check_errors=True)
         want = ref.batch_reference(dict(k=k, v=v, table=far), lens, [3], q, 1 / math.sqrt(dim))
         ref.check_attention(out, lse, want, BF, rows * group <= 16)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-44])
+def test_container_prefix_scales(ctx, scale):
+    import kvexp_amd as kv
+
+    g = gen(47)
+    lens, tokens, dim = [30, 0], 500, 64
+    c = ref.make_batch(g, lens, [1, 1], 16, 2, dim, BF)
+    pk, pv = prefix_kv(g, 2, tokens, dim, "escapes")
+    prefix = ctx.prefix(encode(ctx, pk, 100), encode(ctx, pv, 100))
+    cache = kv.PagedCache(ctx, 2, dim, c["k"].shape[0], 16, BF, k=c["k"], v=c["v"])
+    q = torch.randn(2, 6, dim, generator=g).to(BF).cuda()
+    say("prefix scale", scale)
+    out, lse = cache.attention(q, kv.Batch(c["table"], c["lens"]), scale, prefix=prefix, return_lse=True)
+    both = tuple(x.double().cpu().transpose(0, 1) for x in (pk, pv))
+    ref.check_attention(out, lse, ref.batch_reference(c, lens, [1, 1], q, scale, both), BF, False)
