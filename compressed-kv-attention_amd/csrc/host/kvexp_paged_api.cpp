@@ -530,7 +530,12 @@ int kvexp_hip_paged_attention(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, 
                               uint32_t *d_status, void *stream) {
     return guarded([&] {
         const char *who = "kvexp_hip_paged_attention";
-        if (!std::isfinite(scale)) bad(std::string(who) + ": the scale is not finite");
+        // never 0, which times a masked place's -inf is no number: the least
+        // normal number instead (with products q . k up to 2^100 the weights
+        // are those of scale 0 to 2^-26)
+        float scale2 = float(double(scale) * 1.4426950408889634074);
+        if (!std::isfinite(scale2)) bad(std::string(who) + ": the scale is not finite, or past float's range");
+        if (std::fabs(scale2) < FLT_MIN) scale2 = std::copysign(FLT_MIN, scale2);
         if (d_status == nullptr) bad(std::string(who) + ": null status word");
         if (batch != nullptr && batch->n_tokens > 0) {
             check_rows(who, "q", q);
@@ -542,12 +547,6 @@ int kvexp_hip_paged_attention(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, 
             bad(std::string(who) + ": the workspace must be 16-byte aligned");
         if (workspace_bytes < c.bytes)
             fail(KVEXP_HIP_CAPACITY, std::string(who) + ": workspace below kvexp_hip_paged_attention_workspace");
-        // never 0, which times a masked place's -inf is no number: the least
-        // normal number instead (with products q . k up to 2^100 the weights
-        // are those of scale 0 to 2^-26)
-        float scale2 = float(double(scale) * 1.4426950408889634074);
-        if (!std::isfinite(scale2)) bad(std::string(who) + ": the scale is past float's range");
-        if (std::fabs(scale2) < FLT_MIN) scale2 = std::copysign(FLT_MIN, scale2);
         auto *w = static_cast<uint8_t *>(workspace);
         PagedAttnArgs &a = c.own;
         a.q = rows_in(q);

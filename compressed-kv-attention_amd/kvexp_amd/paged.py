@@ -342,11 +342,12 @@ class PagePrefix:
 
 class PagedCache:
     """Pages of keys and values: k and v [n_pages, n_heads, page_tokens, head_dim] (given, in any strides that are
-    multiples of 8 elements with contiguous channels, or made here)."""
+    multiples of 8 elements with contiguous channels, or made here). status: an int32 word on the device for the errors
+    that only the device can see (None: one of its own)."""
 
-    def __init__(self, ctx, n_heads: int, dim: int, n_pages: int, page_tokens: int = 64, dtype=None, k=None, v=None):
-        import torch
-
+    def __init__(self, ctx, n_heads: int, dim: int, n_pages: int, page_tokens: int = 64, dtype=None, k=None, v=None,
+                 status=None):
+        torch = _torch_module()
         who = "kvexp.PagedCache"
         dtype = torch.bfloat16 if dtype is None else dtype
         self._code = _dtype_code(who, dtype)
@@ -365,13 +366,15 @@ class PagedCache:
             if t.stride(3) != 1 or any(t.stride(i) % 8 for i in range(3)) or t.data_ptr() % 16:
                 raise ValueError(f"{who}: {name} must have contiguous channels, strides of multiples of 8 elements and "
                                  "16-byte alignment")
-        _check_device(who, ctx.device, k=k, v=v)
+        if status is not None and (status.dtype is not torch.int32 or status.numel() != 1):
+            raise ValueError(f"{who}: status must be one int32 word")
+        _check_device(who, ctx.device, k=k, v=v, status=status)
         dev = torch.device("cuda", ctx.device)
         self.ctx, self.dtype = ctx, dtype
         self.n_pages, self.n_heads, self.page_tokens, self.dim = shape
         self.k = torch.empty(shape, dtype=dtype, device=dev) if k is None else k
         self.v = torch.empty(shape, dtype=dtype, device=dev) if v is None else v
-        self.status_word = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.status_word = torch.zeros(1, dtype=torch.int32, device=dev) if status is None else status
         self._sizes = {}
         sk, sv = self.k.stride(), self.v.stride()
         self._struct = _Pages(self.k.data_ptr(), self.v.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],

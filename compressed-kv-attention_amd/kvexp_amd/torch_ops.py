@@ -27,6 +27,7 @@ trace under torch.compile / FakeTensorMode without a GPU.
 """
 from __future__ import annotations
 
+import itertools
 from collections import OrderedDict
 
 import torch
@@ -321,12 +322,8 @@ def _paged(k_pages: Tensor, v_pages: Tensor, status: Tensor) -> PagedCache:
         raise ValueError("kvexp.paged: the pages must be ROCm device tensors")
     if k_pages.dim() != 4:
         raise ValueError("kvexp.paged: pages must be [n_pages, n_heads, page_tokens, head_dim]")
-    if status.dtype != torch.int32 or status.numel() != 1 or status.device != k_pages.device:
-        raise ValueError("kvexp.paged: status must be an int32 word on the pages' device")
     p, h, t, d = k_pages.shape
-    cache = PagedCache(_context(k_pages.device), h, d, p, t, k_pages.dtype, k=k_pages, v=v_pages)
-    cache.status_word = status
-    return cache
+    return PagedCache(_context(k_pages.device), h, d, p, t, k_pages.dtype, k_pages, v_pages, status)
 
 
 @torch.library.custom_op("kvexp::paged_append", mutates_args=("k_pages", "v_pages", "status"))
@@ -362,13 +359,15 @@ def _(k_pages, v_pages, status, q, table, lens, starts, scale, max_new=0, max_le
 
 
 _prefixes: dict[int, Prefix] = {}
+_handles = itertools.count(1)  # a handle is not given twice
 
 
 def register_prefix(ks: list, vs: list) -> int:
     """Registers containers (one K and one V per KV head, on one device) as a shared prefix for
     torch.ops.kvexp.prefix_attention; returns the handle. They must not change while registered."""
-    h = 1 + max(_prefixes, default=0)
-    _prefixes[h] = _context(ks[0].blob.device).prefix(ks, vs)
+    p = _context(ks[0].blob.device).prefix(ks, vs)
+    h = next(_handles)
+    _prefixes[h] = p
     return h
 
 
