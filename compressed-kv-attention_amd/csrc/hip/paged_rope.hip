@@ -255,8 +255,16 @@ using namespace kvexp_dev;
 hipError_t rotate(RotateArgs a, bool half, hipStream_t s) {
     using namespace kvexp_dev::paged;
     if (a.n_tokens <= 0) return hipSuccess;
-    // several tokens per workgroup once there are workgroups for every CU
-    a.tokens_per_group = std::max(1, std::min(kRotTokens, a.n_tokens / 2048));
+    // Four tokens per workgroup once there are workgroups for every CU (32,760
+    // tokens x 12 heads x 128 channels: 38 us; one token 55, two 46, eight 41,
+    // sixteen 48, whose one round of workgroups makes its tables all at once
+    // and then streams), more where four are less than a unit per thread
+    // (200,000 tokens of one head of 64 channels: 23 us, with four tokens 44).
+    const int64_t units = (int64_t(a.n_q) + 2 * a.n_kv) * a.dim / 16; // (about)
+    a.tokens_per_group = std::max(1, std::min(4, a.n_tokens / 2048));
+    while (2 * a.tokens_per_group <= kRotTokens && a.tokens_per_group * units < kRotThreads &&
+           a.n_tokens / (2 * a.tokens_per_group) >= 2048)
+        a.tokens_per_group *= 2;
     const unsigned groups = unsigned((a.n_tokens + a.tokens_per_group - 1) / a.tokens_per_group);
     const size_t lds = size_t(a.tokens_per_group) * size_t(std::max(1, a.rope.n_freq)) * sizeof(float2);
     const int nf = a.rope.n_freq;

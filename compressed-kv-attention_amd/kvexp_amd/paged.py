@@ -121,9 +121,10 @@ def _check_rows(who: str, name: str, t, dtype, n=None, heads=None, dim=None) -> 
         raise ValueError(f"{who}: {name} must be {[n, heads, dim]}, not {list(shape)}")
 
 
-def _check_device(who: str, device: int, **tensors) -> None:
-    for name, t in tensors.items():
+def _check_device(who: str, device: int, *tensors, names) -> None:
+    for t in tensors:
         if t is not None and t.get_device() != device:  # (-1: not on a GPU)
+            name = next(n for n, x in zip(names, tensors) if x is t)
             raise ValueError(f"{who}: {name} must be on cuda:{device}, not {t.device}")
 
 
@@ -199,7 +200,7 @@ class Rope:
         self.interleaved, self.scale = bool(interleaved), float(scale)
 
     def _struct(self, who: str, device: int, dim: int, n_axes: int) -> _Rope:
-        _check_device(who, device, inv_freq=self.inv_freq, axes=self.axes)
+        _check_device(who, device, self.inv_freq, self.axes, names=("inv_freq", "axes"))
         n = int(self.inv_freq.numel())
         if 2 * n > dim:
             raise ValueError(f"{who}: {2 * n} rotated channels, head_dim {dim}")
@@ -218,7 +219,7 @@ def _positions(who: str, device: int, positions, offset: int, n: int):
     wide = positions.dtype is torch.int64
     if not wide and positions.dtype is not torch.int32:
         raise ValueError(f"{who}: positions must be int32 or int64")
-    _check_device(who, device, positions=positions)
+    _check_device(who, device, positions, names=("positions",))
     axes = 1 if len(shape) == 1 else int(shape[0])
     if positions.stride(-1) != 1 or (axes > 1 and positions.stride(0) < n):
         positions = positions.contiguous()
@@ -236,7 +237,7 @@ def rope(ctx, x, positions, rope: Rope, out=None, inverse: bool = False, stream=
         raise ValueError(f"{who}: head_dim must be a multiple of 8 and at most 256")
     if out is not None:
         _check_rows(who, "out", out, x.dtype, n, heads, dim)
-    _check_device(who, ctx.device, x=x, out=out)
+    _check_device(who, ctx.device, x, out, names=("x", "out"))
     if stream is not None:
         with _on(stream):
             return globals()["rope"](ctx, x, positions, rope, out, inverse)
@@ -244,7 +245,7 @@ def rope(ctx, x, positions, rope: Rope, out=None, inverse: bool = False, stream=
     at, axes, keep = _positions(who, ctx.device, positions, 0, n)
     r = rope._struct(who, ctx.device, dim, axes)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(x.shape)
     to = _writable(who, "out", out)
     if n and heads:
         src, x = _readable(x)
@@ -266,26 +267,22 @@ class Batch:
     def __init__(self, table, lens, starts=None, max_new: int | None = None, max_len: int | None = None):
         who, i32 = "kvexp.Batch", _torch_module().int32
         for name, t, d in (("table", table, 2), ("lens", lens, 1), ("starts", starts, 1)):
-            if t is not None and (t.dim() != d or t.dtype is not i32):
+            if t is not None and (t.dtype is not i32 or t.dim() != d):
                 raise ValueError(f"{who}: {name} must be int32 with {d} dimension{'s' if d > 1 else ''}")
-        n = int(lens.shape[0])
-        if table.shape[0] != n or (starts is not None and starts.shape[0] != n + 1):
+        n, (rows, width) = lens.shape[0], table.shape
+        if rows != n or (starts is not None and starts.shape[0] != n + 1):
             raise ValueError(f"{who}: table and lens have one row per sequence, starts one more")
-        self.table = table if table.stride(1) == 1 or table.shape[1] <= 1 else table.contiguous()
+        self.table = table if width <= 1 or table.stride(1) == 1 else table.contiguous()
         self.lens, self.starts = lens.contiguous(), None if starts is None else starts.contiguous()
-        self.max_new, self.max_len = max_new, max_len
-
-    @property
-    def n_seqs(self) -> int:
-        return int(self.lens.shape[0])
+        self.max_new, self.max_len, self.n_seqs = max_new, max_len, n
 
     def _struct(self, who: str, device: int, n_tokens: int) -> _Batch:
-        _check_device(who, device, table=self.table, lens=self.lens, starts=self.starts)
-        if self.starts is None and (n_tokens % self.n_seqs if self.n_seqs else n_tokens):
-            raise ValueError(f"{who}: {n_tokens} tokens of {self.n_seqs} sequences without starts")
-        return _Batch(self.table.data_ptr(), self.lens.data_ptr(),
-                      None if self.starts is None else self.starts.data_ptr(), self.table.stride(0),
-                      int(self.table.shape[1]), self.n_seqs, n_tokens, int(self.max_new or 0), int(self.max_len or 0), 0)
+        table, lens, starts, n = self.table, self.lens, self.starts, self.n_seqs
+        _check_device(who, device, table, lens, starts, names=("table", "lens", "starts"))
+        if starts is None and (n_tokens % n if n else n_tokens):
+            raise ValueError(f"{who}: {n_tokens} tokens of {n} sequences without starts")
+        return _Batch(table.data_ptr(), lens.data_ptr(), None if starts is None else starts.data_ptr(), table.stride(0),
+                      table.shape[1], n, n_tokens, int(self.max_new or 0), int(self.max_len or 0))
 
 
 class Prefix:
@@ -336,7 +333,7 @@ class PagePrefix:
     def _struct(self, who: str, cache) -> _Shared:
         if cache is not self.cache:
             raise ValueError(f"{who}: the prefix is in pages of another cache")
-        _check_device(who, cache.ctx.device, prefix=self.table)
+        _check_device(who, cache.ctx.device, self.table, names=("prefix",))
         return _Shared(None, self.table.data_ptr(), int(self.table.shape[0]), self.seq)
 
 
@@ -368,7 +365,7 @@ class PagedCache:
                                  "16-byte alignment")
         if status is not None and (status.dtype is not torch.int32 or status.numel() != 1):
             raise ValueError(f"{who}: status must be one int32 word")
-        _check_device(who, ctx.device, k=k, v=v, status=status)
+        _check_device(who, ctx.device, k, v, status, names=("k", "v", "status"))
         dev = torch.device("cuda", ctx.device)
         self.ctx, self.dtype = ctx, dtype
         self.n_pages, self.n_heads, self.page_tokens, self.dim = shape
@@ -401,7 +398,7 @@ class PagedCache:
             if q is None:
                 raise ValueError(f"{who}: q and q_out go together")
             _check_rows(who, "q_out", q_out, self.dtype, *q.shape)
-        _check_device(who, self.ctx.device, k=k, v=v, q=q, q_out=q_out)
+        _check_device(who, self.ctx.device, k, v, q, q_out, names=("k", "v", "q", "q_out"))
         if stream is not None:
             with _on(stream):
                 return self.append(k, v, batch, rope, positions, offset, q, q_out, check_errors)
@@ -410,7 +407,7 @@ class PagedCache:
         r = None if rope is None else rope._struct(who, self.ctx.device, self.dim, axes)
         b = batch._struct(who, self.ctx.device, n)
         if q is not None and q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out = q.new_empty(q.shape)
         to = None if q is None else _writable(who, "q_out", q_out)
         if n:
             (kr, k), (vr, v) = _readable(k), _readable(v)
@@ -442,7 +439,7 @@ class PagedCache:
         scale = 1.0 / math.sqrt(self.dim) if scale is None else float(scale)
         if not math.isfinite(scale):
             raise ValueError(f"{who}: the scale is not finite")
-        _check_device(who, self.ctx.device, q=q, out=out, lse=lse)
+        _check_device(who, self.ctx.device, q, out, lse, names=("q", "out", "lse"))
         if stream is not None:
             with _on(stream):
                 return self.attention(q, batch, scale, prefix, out, lse, return_lse, check_errors)
@@ -450,12 +447,12 @@ class PagedCache:
         b = batch._struct(who, self.ctx.device, n)
         sh = None if prefix is None else prefix._struct(who, self)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = q.new_empty(q.shape)
         to = _writable(who, "out", out)
         if lse is None and return_lse:
             lse = torch.empty((n, heads), dtype=torch.float32, device=q.device)
         # the workspace follows the sizes of the call
-        key = (n, heads, b.n_seqs, b.table_width, b.starts is None, b.max_new, b.max_len,
+        key = (n, heads, batch.n_seqs, batch.table.shape[1], batch.starts is None, batch.max_new, batch.max_len,
                None if sh is None else (sh.xkv is None, sh.n_tokens))
         size = self._sizes.get(key)
         if size is None:
