@@ -168,10 +168,21 @@ Cut cut_of(const kvexp_hip_ctx *ctx, int64_t rows, int64_t pairs, int max_len, i
     const bool many = coded || rows > few_rows(dim);
     c.tile_rows = !many ? (rows > 16 ? 32 : 16) : rows > 128 ? many_rows(dim, coded) : 128;
     c.row_tiles = int((rows + c.tile_rows - 1) / c.tile_rows);
-    c.min_split = 256;
-    const int64_t target = int64_t(std::max(1, ctx->cu_count)) * (many ? (c.tile_rows == 256 ? 1 : 2) : 8);
+    // Few rows: splits of 512 tokens at least (one sequence of 65,536 tokens, 2
+    // heads of 64 channels: 23.6 us, with 256 31.7) and eight workgroups per CU
+    // in all, of which three run at once, so that short sequences' empty splits
+    // leave enough of them (64 sequences of 1K to 32K: 85 us, with five 90,
+    // with sixteen 79; but four of up to 65,536 at 128 channels 125, 123, 136);
+    // with two products of rows six, as every split's states cost twice as
+    // much (16 sequences of 8,192, 32 rows of 128 channels: 77 us, with eight
+    // 83, with four 73; but of 1K to 8K at 96 channels 54, 56, 64). Many rows:
+    // 256 at least (30 rows over 4,096 compressed tokens: 25 us, with 512 33),
+    // and the workgroups that are resident.
+    c.min_split = many ? 256 : 512;
+    const int64_t per_cu = !many ? (c.tile_rows == 32 ? 6 : 8) : c.tile_rows == 256 ? 1 : 2;
+    const int64_t target = int64_t(std::max(1, ctx->cu_count)) * per_cu;
     const int64_t base = std::max<int64_t>(1, pairs * c.row_tiles);
-    // (many rows: the workgroups that are resident, no second round for a few more)
+    // (many rows: no second round for a few more)
     const int64_t want = many ? std::max<int64_t>(1, target / base) : (target + base - 1) / base;
     const int64_t most = std::max<int64_t>(1, (int64_t(max_len) + c.min_split - 1) / c.min_split);
     c.n_splits = int(std::max<int64_t>(1, std::min<int64_t>({want, most, 256})));
