@@ -388,7 +388,8 @@ void build_prefix(kvexp_hip_prefix &p, const kvexp_hip_head *heads, hipStream_t 
                  o_blocks = o_jobs + padded(jobs_b), o_e0 = o_blocks + padded(blocks.size() * sizeof(int2)),
                  o_segs = o_e0 + padded(total * sizeof(int32_t)),
                  o_pos = o_segs + padded(segs.size() * sizeof(PrefixSeg));
-    const size_t pos_b = std::max<size_t>(1, pos_total) * sizeof(uint32_t);
+    // (and one more: a run without records reads the one where its own would be)
+    const size_t pos_b = (pos_total + 1) * sizeof(uint32_t);
     p.arena = DevBuf(o_pos + pos_b);
     uint8_t *d = p.arena.as<uint8_t>();
     std::vector<uint8_t> image(o_pos, 0); // (the status word 0)
