@@ -673,11 +673,17 @@ __device__ __forceinline__ int thread_here() {
 //
 // Bound: the vector ALU (per tile and wave 32 exponentials at a quarter of its
 // rate, their arguments, maxima and sums) and the matrix cores, in turn. The
-// tile after next is on its way in registers and the next one in the other
-// half of LDS while a tile is worked on; a workgroup's waves meet once per tile
-// (containers: twice, the escapes being written over their elements between),
-// and two workgroups share a CU, so that one's products run beside the other's
-// exponentials.
+// tile after next is on its way in registers and the next one in another part
+// of LDS while a tile is worked on; a workgroup's waves meet once per tile
+// (containers in two parts: twice, the escapes being written over their
+// elements between). Four waves of two workgroups share a CU, or eight of one,
+// two per SIMD, so that one's products run beside the other's exponentials.
+// Measured: chunks of prompts (8 sequences, 32 heads of 128 channels) 0.9
+// PFLOP/s in 573 us, the matrix cores busy 45 % of it and the vector ALU 51 %;
+// four waves per workgroup 665, a maximum per 32 tokens 860. 256 rows over
+// 65,536 compressed tokens of 8 heads of 128 channels: 138 us (matrix cores 23
+// %, vector ALU 37 %; with the decode's two barriers per tile 140 to 143, with
+// two tiles on their way, which spills at 128 channels, 175).
 template <int DP, int NW>
 struct Many {
     static constexpr int T = 64 * NW;                         // threads
@@ -702,10 +708,14 @@ struct alignas(16) ManyBuf {
     uint16_t k[Many<DP, 4>::KT * Many<DP, 4>::KR];
     uint16_t v[Many<DP, 4>::KT * Many<DP, 4>::VR];
 };
-template <int DP>
+// Pages: two halves, and where K and V of the tokens of tiles on their way
+// begin (bytes). Containers: three parts where the LDS of the workgroups of a
+// CU allows it, else two.
+template <int DP, int SRC, int NW>
 struct alignas(16) ManyLds {
-    ManyBuf<DP> buf[2];
-    longlong2 row[2][Many<DP, 4>::KT]; // where K and V of the tokens of tiles on their way begin (bytes)
+    static constexpr int Bufs = SRC == 1 && (NW == 8 || DP <= 64 || DP > 128) ? 3 : 2;
+    ManyBuf<DP> buf[Bufs];
+    longlong2 row[2][SRC == 0 ? Many<DP, 4>::KT : 1];
 };
 
 typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
@@ -935,7 +945,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(Many<DP
 paged_many_kernel(PagedAttnArgs a) {
     using S = Many<DP, NW>;
     extern __shared__ __align__(16) uint8_t many_lds[];
-    ManyLds<DP> &lds = *reinterpret_cast<ManyLds<DP> *>(many_lds);
+    using Lds = ManyLds<DP, SRC, NW>;
+    Lds &lds = *reinterpret_cast<Lds *>(many_lds);
     const int tid = int(threadIdx.x), lane = lane_id(), wave = tid >> 6, c = lane & 31, h = lane >> 5;
     int split, head, tile, seq;
     find_work(a, split, head, tile, seq);
@@ -951,7 +962,7 @@ paged_many_kernel(PagedAttnArgs a) {
     const uint16_t *kh = a.pool.k + int64_t(head) * a.pool.k_head;
     const uint16_t *vh = a.pool.v + int64_t(head) * a.pool.v_head;
     // channels past head_dim: K's are zero (they meet zero queries), V's feed outputs that nobody reads
-    for (int i = tid; i < 2 * S::KT * (DP - a.dim); i += S::T) {
+    for (int i = tid; i < Lds::Bufs * S::KT * (DP - a.dim); i += S::T) {
         const int t = i / (DP - a.dim), d = a.dim + i - t * (DP - a.dim), b = t / S::KT;
         lds.buf[b].k[(t - b * S::KT) * S::KR + d] = 0;
         lds.buf[b].v[(t - b * S::KT) * S::VR + d] = 0;
@@ -1221,15 +1232,40 @@ paged_many_kernel(PagedAttnArgs a) {
             int t = r.t0 / S::KT;
             fetch(t);
             request(t);
-            for (int tok = r.t0, b = 0; tok < r.t1; tok += S::KT, ++t, b ^= 1) {
-                coded_store<DP, NW, S::KR, false>(k0, ks, a.dim, at, kt, lds.buf[b].k);
-                coded_store<DP, NW, S::VR, true>(v0, vs, a.dim, at, vt, lds.buf[b].v);
-                team::team_sync(); // (as below: loads on their way stay on their way)
-                coded_patch<DP, NW, S::KR>(k0, ks, a.dim, kt, lds.buf[b].k);
-                coded_patch<DP, NW, S::VR>(v0, vs, a.dim, vt, lds.buf[b].v);
-                if (tok + S::KT < r.t1) request(t + 1);
+            auto put = [&](ManyBuf<DP> &buf) {
+                coded_store<DP, NW, S::KR, false>(k0, ks, a.dim, at, kt, buf.k);
+                coded_store<DP, NW, S::VR, true>(v0, vs, a.dim, at, vt, buf.v);
+            };
+            auto patch = [&](ManyBuf<DP> &buf, bool more) { // and the next tile's rows requested
+                coded_patch<DP, NW, S::KR>(k0, ks, a.dim, kt, buf.k);
+                coded_patch<DP, NW, S::VR>(v0, vs, a.dim, vt, buf.v);
+                if (more) request(++t);
+            };
+            // (team_sync: loads on their way stay on their way)
+            if constexpr (Lds::Bufs == 3) {
+                // The part that the next tile is put in was last read two tiles
+                // ago, and its escapes are written before the barrier that the
+                // tile's own work waits for: one barrier per tile.
+                put(lds.buf[0]);
                 team::team_sync();
-                if (busy) work(Cut{}, tok, lds.buf[b], false);
+                patch(lds.buf[0], r.t0 + S::KT < r.t1);
+                for (int tok = r.t0, b = 0; tok < r.t1; tok += S::KT) {
+                    const int next = b == 2 ? 0 : b + 1;
+                    const bool more = tok + S::KT < r.t1;
+                    if (more) put(lds.buf[next]);
+                    team::team_sync();
+                    if (more) patch(lds.buf[next], tok + 2 * S::KT < r.t1);
+                    if (busy) work(Cut{}, tok, lds.buf[b], false);
+                    b = next;
+                }
+            } else {
+                for (int tok = r.t0, b = 0; tok < r.t1; tok += S::KT, b ^= 1) {
+                    put(lds.buf[b]);
+                    team::team_sync();
+                    patch(lds.buf[b], tok + S::KT < r.t1);
+                    team::team_sync();
+                    if (busy) work(Cut{}, tok, lds.buf[b], false);
+                }
             }
         }
     }

@@ -30,14 +30,15 @@ void launch_few(const PagedAttnArgs &a, bool two, int n_seqs, hipStream_t s) {
 template <int DP, bool HALF, int SRC, int NW>
 hipError_t launch_many_waves(const PagedAttnArgs &a, int n_seqs, hipStream_t s) {
     // (past the default 64 KiB of LDS; the attribute is a device's own, so every call sets it)
-    if (sizeof(ManyLds<DP>) > 64 * 1024) {
+    constexpr size_t lds = sizeof(ManyLds<DP, SRC, NW>);
+    if (lds > 64 * 1024) {
         const hipError_t set =
             hipFuncSetAttribute(reinterpret_cast<const void *>(paged_many_kernel<DP, HALF, SRC, NW>),
-                                hipFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(ManyLds<DP>)));
+                                hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
         if (set != hipSuccess) return set;
     }
     hipLaunchKernelGGL((paged_many_kernel<DP, HALF, SRC, NW>), attention_grid(a, n_seqs), dim3(64 * NW),
-                       sizeof(ManyLds<DP>), s, a);
+                       lds, s, a);
     return hipGetLastError();
 }
 
