@@ -678,8 +678,9 @@ __device__ __forceinline__ int thread_here() {
 // (containers in two parts: twice, the escapes being written over their
 // elements between). Four waves of two workgroups share a CU, or eight of one,
 // two per SIMD, so that one's products run beside the other's exponentials.
-// Measured: chunks of prompts (8 sequences, 32 heads of 128 channels) 0.9
-// PFLOP/s in 573 us, the matrix cores busy 45 % of it and the vector ALU 51 %;
+// Measured: chunks of two prompts (of up to 2,048 tokens, up to 16,384 seen, 32
+// heads of 128 channels) 0.9 PFLOP/s in 573 us, the matrix cores busy 45 % of it
+// and the vector ALU 51 %;
 // four waves per workgroup 665, a maximum per 32 tokens 860. 256 rows over
 // 65,536 compressed tokens of 8 heads of 128 channels: 138 us (matrix cores 23
 // %, vector ALU 37 %; with the decode's two barriers per tile 140 to 143, with

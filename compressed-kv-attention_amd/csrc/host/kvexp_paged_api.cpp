@@ -22,7 +22,7 @@ hipError_t prefix_segs(PrefixSeg *segs, int n, const EscJob *jobs, hipStream_t s
 } // namespace kvexp_launch
 
 struct kvexp_hip_prefix {
-    kvexp_hip_ctx *ctx = nullptr;
+    int device = 0; // (the context may be gone when the prefix goes)
     int n_heads = 0, dim = 0, seq = 0;
     DevBuf arena;
     const PrefixTensor *tensors = nullptr;
@@ -169,16 +169,18 @@ Cut cut_of(const kvexp_hip_ctx *ctx, int64_t rows, int64_t pairs, int max_len, i
     c.tile_rows = !many ? (rows > 16 ? 32 : 16) : rows > 128 ? many_rows(dim, coded) : 128;
     c.row_tiles = int((rows + c.tile_rows - 1) / c.tile_rows);
     // Few rows: splits of 512 tokens at least (one sequence of 65,536 tokens, 2
-    // heads of 64 channels: 23.6 us, with 256 31.7) and eight workgroups per CU
-    // in all, of which three run at once, so that short sequences' empty splits
-    // leave enough of them (64 sequences of 1K to 32K: 85 us, with five 90,
-    // with sixteen 79; but four of up to 65,536 at 128 channels 125, 123, 136);
-    // with two products of rows six, as every split's states cost twice as
-    // much (16 sequences of 8,192, 32 rows of 128 channels: 77 us, with eight
-    // 83, with four 73; but of 1K to 8K at 96 channels 54, 56, 64). Many rows:
-    // 256 at least (30 rows over 4,096 compressed tokens: 25 us, with 512 33),
-    // and the workgroups that are resident.
-    c.min_split = many ? 256 : 512;
+    // heads of 64 channels: 23.6 us, with 256 31.7), where that leaves eight of
+    // them (one of 1,021 tokens: kernels 11.8 us with 256, 12.9 with 512); eight
+    // workgroups per CU in all, of which three run at once, so that short
+    // sequences' empty splits leave enough of them (64 sequences of 1K to 32K:
+    // 85 us, with five 90, with sixteen 79; but four of up to 65,536 at 128
+    // channels 125, 123, 136); with two products of rows six, as every split's
+    // states cost twice as much (16 sequences of 8,192, 32 rows of 128 channels:
+    // 77 us, with eight 83, with four 73; but 16 of up to 16,411 with up to five
+    // drafts, 4 queries of 96 channels: 54, 56, 64). Many rows: 256 at least (30
+    // rows over 4,096 compressed tokens: 25 us, with 512 33), and the workgroups
+    // that are resident.
+    c.min_split = many || max_len <= 4096 ? 256 : 512;
     const int64_t per_cu = !many ? (c.tile_rows == 32 ? 6 : 8) : c.tile_rows == 256 ? 1 : 2;
     const int64_t target = int64_t(std::max(1, ctx->cu_count)) * per_cu;
     const int64_t base = std::max<int64_t>(1, pairs * c.row_tiles);
@@ -243,7 +245,7 @@ Call plan_call(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, const kvexp_hip
     }
     if (a.batch.n_tokens == 0) return c;
     if (ctx == nullptr) bad(std::string(who) + ": null context");
-    if (c.has_shared && shared->xkv != nullptr && shared->xkv->ctx->device != ctx->device)
+    if (c.has_shared && shared->xkv != nullptr && shared->xkv->device != ctx->device)
         bad(std::string(who) + ": the prefix is on another device");
     const int64_t rows = int64_t(a.batch.max_new) * a.group;
     c.cut = cut_of(ctx, rows, int64_t(a.batch.n_seqs) * a.n_kv, max_len, a.dim, false);
@@ -294,7 +296,7 @@ Call plan_call(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, const kvexp_hip
 // The tables of a prefix kept as containers: reads the block indexes (checked
 // block by block), cuts every tensor's tokens into the kernel's tiles and
 // those at block ends, and fills in addresses and escape records on the GPU.
-void build_prefix(kvexp_hip_prefix &p, const kvexp_hip_head *heads, hipStream_t s) {
+void build_prefix(kvexp_hip_ctx *ctx, kvexp_hip_prefix &p, const kvexp_hip_head *heads, hipStream_t s) {
     const int n = 2 * p.n_heads, kt = tile_tokens(p.dim);
     std::vector<EscJob> jobs;
     std::vector<size_t> at; // a tensor's first entry in the index arrays
@@ -320,7 +322,7 @@ void build_prefix(kvexp_hip_prefix &p, const kvexp_hip_head *heads, hipStream_t 
     };
     const size_t jobs_b = jobs.size() * sizeof(EscJob);
     {
-        DevBuf buf(&p.ctx->pool, jobs_b + (1 + 2 * total) * sizeof(int32_t));
+        DevBuf buf(&ctx->pool, jobs_b + (1 + 2 * total) * sizeof(int32_t));
         auto *words = reinterpret_cast<int32_t *>(buf.as<uint8_t>() + jobs_b);
         std::vector<uint8_t> up(jobs_b + sizeof(uint32_t), 0);
         SyncOnExit sync{s};
@@ -332,7 +334,7 @@ void build_prefix(kvexp_hip_prefix &p, const kvexp_hip_head *heads, hipStream_t 
         }
         HIPX(hipMemcpyAsync(buf.p, up.data(), up.size(), hipMemcpyHostToDevice, s));
         HIPX(kvexp_launch::esc_start(buf.as<EscJob>(), n, reinterpret_cast<uint32_t *>(words), s));
-        auto *host = static_cast<int32_t *>(pinned_staging(p.ctx, (1 + 2 * total) * sizeof(int32_t)));
+        auto *host = static_cast<int32_t *>(pinned_staging(ctx, (1 + 2 * total) * sizeof(int32_t)));
         HIPX(hipMemcpyAsync(host, words, (1 + 2 * total) * sizeof(int32_t), hipMemcpyDeviceToHost, s));
         HIPX(hipStreamSynchronize(s));
         if (host[0] != 0) fail(KVEXP_HIP_FORMAT_ERROR, status_message(uint32_t(host[0])));
@@ -412,7 +414,7 @@ void build_prefix(kvexp_hip_prefix &p, const kvexp_hip_head *heads, hipStream_t 
     const auto *dj = reinterpret_cast<const EscJob *>(d + o_jobs);
     HIPX(kvexp_launch::esc_pos(dj, reinterpret_cast<const int2 *>(d + o_blocks), int(blocks.size()), st, s));
     HIPX(kvexp_launch::prefix_segs(reinterpret_cast<PrefixSeg *>(d + o_segs), int(segs.size()), dj, s));
-    check_status_word(p.ctx, st, s);
+    check_status_word(ctx, st, s);
     p.tensors = reinterpret_cast<const PrefixTensor *>(d + o_tensors);
 }
 
@@ -507,11 +509,11 @@ int kvexp_hip_prefix_create(kvexp_hip_ctx *ctx, const kvexp_hip_head *heads, int
         DeviceGuard g(ctx->device);
         auto *p = new kvexp_hip_prefix();
         try {
-            p->ctx = ctx;
+            p->device = ctx->device;
             p->n_heads = n_heads;
             p->dim = dim;
             p->seq = seq;
-            build_prefix(*p, heads, static_cast<hipStream_t>(stream));
+            build_prefix(ctx, *p, heads, static_cast<hipStream_t>(stream));
         } catch (...) {
             delete p;
             throw;
@@ -523,7 +525,7 @@ int kvexp_hip_prefix_create(kvexp_hip_ctx *ctx, const kvexp_hip_head *heads, int
 int kvexp_hip_prefix_destroy(kvexp_hip_prefix *prefix) {
     return guarded([&] {
         if (prefix == nullptr) return;
-        DeviceGuard g(prefix->ctx->device);
+        DeviceGuard g(prefix->device);
         delete prefix;
     });
 }

@@ -179,6 +179,11 @@ def _raw_stream(device: int) -> int:
     return _torch_module()._C._cuda_getCurrentRawStream(device)
 
 
+def _read_only(name: str):
+    """A property without a setter: what was checked when the object was made stays what the calls use."""
+    return property(lambda self: getattr(self, name))
+
+
 class Rope:
     """A rotation of the first 2 n channels of a row.
 
@@ -196,16 +201,19 @@ class Rope:
             raise ValueError("kvexp.Rope: axes must be uint8, one per frequency")
         if not math.isfinite(scale):
             raise ValueError("kvexp.Rope: the scale is not finite")
-        self.inv_freq, self.axes = inv_freq.contiguous(), None if axes is None else axes.contiguous()
+        self._inv_freq, self._axes = inv_freq.contiguous(), None if axes is None else axes.contiguous()
         self.interleaved, self.scale = bool(interleaved), float(scale)
 
+    inv_freq, axes = _read_only("_inv_freq"), _read_only("_axes")
+
     def _struct(self, who: str, device: int, dim: int, n_axes: int) -> _Rope:
-        _check_device(who, device, self.inv_freq, self.axes, names=("inv_freq", "axes"))
-        n = int(self.inv_freq.numel())
+        inv_freq, axes = self._inv_freq, self._axes
+        _check_device(who, device, inv_freq, axes, names=("inv_freq", "axes"))
+        n = inv_freq.numel()
         if 2 * n > dim:
             raise ValueError(f"{who}: {2 * n} rotated channels, head_dim {dim}")
-        return _Rope(self.inv_freq.data_ptr(), None if self.axes is None else self.axes.data_ptr(), n, n_axes,
-                     int(self.interleaved), self.scale)
+        return _Rope(inv_freq.data_ptr(), None if axes is None else axes.data_ptr(), n, n_axes, int(self.interleaved),
+                     self.scale)
 
 
 def _positions(who: str, device: int, positions, offset: int, n: int):
@@ -272,12 +280,15 @@ class Batch:
         n, (rows, width) = lens.shape[0], table.shape
         if rows != n or (starts is not None and starts.shape[0] != n + 1):
             raise ValueError(f"{who}: table and lens have one row per sequence, starts one more")
-        self.table = table if width <= 1 or table.stride(1) == 1 else table.contiguous()
-        self.lens, self.starts = lens.contiguous(), None if starts is None else starts.contiguous()
-        self.max_new, self.max_len, self.n_seqs = max_new, max_len, n
+        rs, cs = table.stride()
+        self._table = table if (width <= 1 or cs == 1) and (n <= 1 or rs >= width) else table.contiguous()
+        self._lens, self._starts, self._n_seqs = lens.contiguous(), None if starts is None else starts.contiguous(), n
+        self.max_new, self.max_len = max_new, max_len
+
+    table, lens, starts, n_seqs = (_read_only(x) for x in ("_table", "_lens", "_starts", "_n_seqs"))
 
     def _struct(self, who: str, device: int, n_tokens: int) -> _Batch:
-        table, lens, starts, n = self.table, self.lens, self.starts, self.n_seqs
+        table, lens, starts, n = self._table, self._lens, self._starts, self._n_seqs
         _check_device(who, device, table, lens, starts, names=("table", "lens", "starts"))
         if starts is None and (n_tokens % n if n else n_tokens):
             raise ValueError(f"{who}: {n_tokens} tokens of {n} sequences without starts")
@@ -369,13 +380,15 @@ class PagedCache:
         dev = torch.device("cuda", ctx.device)
         self.ctx, self.dtype = ctx, dtype
         self.n_pages, self.n_heads, self.page_tokens, self.dim = shape
-        self.k = torch.empty(shape, dtype=dtype, device=dev) if k is None else k
-        self.v = torch.empty(shape, dtype=dtype, device=dev) if v is None else v
-        self.status_word = torch.zeros(1, dtype=torch.int32, device=dev) if status is None else status
+        self._k = torch.empty(shape, dtype=dtype, device=dev) if k is None else k
+        self._v = torch.empty(shape, dtype=dtype, device=dev) if v is None else v
+        self._status = torch.zeros(1, dtype=torch.int32, device=dev) if status is None else status
         self._sizes = {}
         sk, sv = self.k.stride(), self.v.stride()
         self._struct = _Pages(self.k.data_ptr(), self.v.data_ptr(), sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
                               self._code, shape[0], shape[2], shape[1], shape[3], 0)
+
+    k, v, status_word = _read_only("_k"), _read_only("_v"), _read_only("_status")
 
     def prefix(self, table, seq: int) -> PagePrefix:
         """The first `seq` tokens of the pages `table` (int32 [pages]) as a prefix that batches share."""
@@ -415,7 +428,7 @@ class PagedCache:
             if q is not None and q.shape[1]:
                 (qr, q), heads = _readable(q), int(q.shape[1])
             _check(L.kvexp_hip_paged_append(self.ctx.h, self._struct, b, kr, vr, r, at, qr, to if heads else None, heads,
-                                            self.status_word.data_ptr(), _raw_stream(self.ctx.device)))
+                                            self._status.data_ptr(), _raw_stream(self.ctx.device)))
         if check_errors:
             self.status()
         return q_out
@@ -452,7 +465,7 @@ class PagedCache:
         if lse is None and return_lse:
             lse = torch.empty((n, heads), dtype=torch.float32, device=q.device)
         # the workspace follows the sizes of the call
-        key = (n, heads, batch.n_seqs, batch.table.shape[1], batch.starts is None, batch.max_new, batch.max_len,
+        key = (n, heads, b.n_seqs, b.table_width, batch._starts is None, batch.max_new, batch.max_len,
                None if sh is None else (sh.xkv is None, sh.n_tokens))
         size = self._sizes.get(key)
         if size is None:
@@ -467,7 +480,7 @@ class PagedCache:
             src, q = _readable(q)
             _check(L.kvexp_hip_paged_attention(
                 self.ctx.h, self._struct, b, sh, src, heads, scale, to, None if lse is None else lse.data_ptr(),
-                None if ws is None else ws.data_ptr(), size, self.status_word.data_ptr(), _raw_stream(self.ctx.device)))
+                None if ws is None else ws.data_ptr(), size, self._status.data_ptr(), _raw_stream(self.ctx.device)))
         if check_errors:
             self.status()
         return (out, lse) if return_lse else out
@@ -475,4 +488,4 @@ class PagedCache:
     def status(self, stream=None) -> None:
         """Raises what the cache's calls found wrong on the device since the last check (synchronises)."""
         kv = _kv()
-        kv.check(kv.lib().kvexp_hip_paged_status(self.ctx.h, self.status_word.data_ptr(), kv._stream(stream)))
+        kv.check(kv.lib().kvexp_hip_paged_status(self.ctx.h, self._status.data_ptr(), kv._stream(stream)))

@@ -430,3 +430,38 @@ def test_rope_traced_and_captured(ctx):
         want = torch.ops.kvexp.rope(e, pos, freq)
         assert torch.equal(out, want) and torch.equal(grad, torch.autograd.grad(want, e, ds)[0])
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("new,longest,dim", [(1, 40, 64), (1, 3000, 64), (6, 700, 128), (70, 80, 64), (70, 3000, 128)])
+def test_outputs_over_the_queries(ctx, new, longest, dim):
+    """out may be q: one split and several, few rows and many."""
+    import kvexp_amd as kv
+
+    g = gen(new + longest)
+    lens, page = [longest, 75], 64
+    c = ref.make_batch(g, lens, [new] * 2, page, 2, dim, BF)
+    q = torch.randn(2 * new, 8, dim, generator=g).to(BF).cuda()
+    cache = kv.PagedCache(ctx, 2, dim, c["k"].shape[0], page, BF, k=c["k"], v=c["v"])
+    batch = kv.Batch(c["table"], c["lens"])
+    say("out over q", new, longest, dim)
+    want = cache.attention(q, batch)
+    assert cache.attention(q, batch, out=q) is q and torch.equal(q, want)
+
+
+def test_tables_of_other_layouts(ctx):
+    """A table in columns, one that every sequence shares by a stride of 0, and a slice of a wider one."""
+    import kvexp_amd as kv
+
+    g = gen(90)
+    lens, page, dim = [150, 90, 33], 64, 64
+    c = ref.make_batch(g, lens, [1] * 3, page, 1, dim, BF)
+    q = torch.randn(3, 4, dim, generator=g).to(BF).cuda()
+    cache = kv.PagedCache(ctx, 1, dim, c["k"].shape[0], page, BF, k=c["k"], v=c["v"])
+    want = cache.attention(q, kv.Batch(c["table"], c["lens"]))
+    wide = torch.full((3, 20), -1, dtype=torch.int32).cuda()
+    wide[:, 5:5 + c["table"].shape[1]] = c["table"]
+    for t in (c["table"].t().contiguous().t(), wide[:, 5:5 + c["table"].shape[1]]):
+        assert torch.equal(want, cache.attention(q, kv.Batch(t, c["lens"])))
+    same = c["table"][:1].expand(3, -1)
+    lens = torch.tensor([150, 90, 33], dtype=torch.int32).cuda()
+    assert torch.equal(cache.attention(q, kv.Batch(same, lens)), cache.attention(q, kv.Batch(same.contiguous(), lens)))

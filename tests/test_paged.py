@@ -212,6 +212,19 @@ def test_caches_refuse():
             kv.PagedCache(CTX, *args, **kw)
 
 
+def test_what_was_checked_stays():
+    """Tensors that a call reads cannot be exchanged for others that nothing has checked."""
+    b = kv.Batch(torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32))
+    r = kv.Rope(torch.zeros(32), torch.zeros(32, dtype=torch.uint8))
+    for o, names in ((b, ("table", "lens", "starts", "n_seqs")), (r, ("inv_freq", "axes"))):
+        for n in names:
+            with pytest.raises(AttributeError):
+                setattr(o, n, getattr(o, n))
+    for n in ("k", "v", "status_word"):
+        with pytest.raises(AttributeError):
+            setattr(object.__new__(kv.PagedCache), n, None)
+
+
 @pytest.fixture
 def cache():
     c = object.__new__(kv.PagedCache)  # (no device to hold its pages)
