@@ -302,7 +302,8 @@ int kvexp_hip_attention_decode_host(kvexp_hip_ctx *ctx, int order, const uint16_
  * Element type: BF16 or FP16 for pages and rows alike; scores, softmax and sums
  * are FP32. head_dim is a multiple of 8, at most 256. Pointers of rows and
  * pages are 16-byte aligned and their strides (in elements) multiples of 8;
- * the channels of a row are contiguous.
+ * the channels of a row are contiguous. A sequence or a shared prefix holds at
+ * most 2^30 tokens; calls whose launch would not fit 2^32 threads are refused.
  *
  * Calls are stream-ordered, allocate nothing and do not synchronise; their
  * lengths, tables and positions are read on the device, so a captured call may
@@ -388,7 +389,7 @@ int kvexp_hip_paged_append(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, con
  * of `seq` tokens (as the heads of a plan; n_splits is not used). Reads the
  * block indexes and builds the tables that the attention kernel needs, ordered
  * on `stream`, which it synchronises. The containers must not change while it
- * lives. */
+ * lives; it may outlive its context, and is destroyed when no call uses it. */
 typedef struct kvexp_hip_prefix kvexp_hip_prefix;
 int kvexp_hip_prefix_create(kvexp_hip_ctx *ctx, const kvexp_hip_head *heads, int n_heads, int dim, void *stream,
                             kvexp_hip_prefix **out);
@@ -409,7 +410,7 @@ typedef struct kvexp_hip_shared {
  * [h g, (h + 1) g) read KV head h, g = n_q_heads / pages->n_heads. out
  * [n_tokens, n_q_heads, dim] is of the pages' type, d_lse (nullable)
  * [n_tokens, n_q_heads] FP32 the log of the sum of exponentials. A token that
- * sees nothing gives 0 and -inf. The workspace (device, 16-byte aligned) holds
+ * sees nothing gives 0 and -inf. out may be q. The workspace (device, 16-byte aligned) holds
  * at least what kvexp_hip_paged_attention_workspace says for the same
  * arguments (-1 where they are refused); calls that overlap need one each. */
 int64_t kvexp_hip_paged_attention_workspace(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages,
