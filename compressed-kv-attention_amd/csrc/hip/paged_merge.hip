@@ -191,9 +191,10 @@ hipError_t prefix_segs(PrefixSeg *segs, int n, const EscJob *jobs, hipStream_t s
 
 hipError_t paged_merge(const PagedAttnArgs &a, bool half, hipStream_t s) {
     const int64_t n = int64_t(a.batch.n_tokens) * a.n_kv * a.group;
-    // four waves per row where the rows alone do not fill the GPU and there
-    // are splits for them
-    const bool four = n < 4096 && a.n_splits + a.s_splits >= 8;
+    // four waves per row where there are splits for them and their workgroups
+    // all run at once (2,048 rows of 32 + 2 splits of 128 channels: 11.3 us, with
+    // one wave 14.5; 3,584 rows of 18 + 1 of 64: 15.0 and 10.9)
+    const bool four = n <= 2048 && a.n_splits + a.s_splits >= 8;
     auto run = [&](auto kernel, int64_t groups) {
         hipLaunchKernelGGL(kernel, dim3(unsigned(groups)), dim3(256), 0, s, a);
     };

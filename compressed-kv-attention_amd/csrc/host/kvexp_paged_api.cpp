@@ -166,7 +166,12 @@ Cut cut_of(const kvexp_hip_ctx *ctx, int64_t rows, int64_t pairs, int max_len, i
     Cut c;
     if (rows > INT32_MAX / 2) fail(KVEXP_HIP_UNSUPPORTED, "paged attention: too many query rows");
     const bool many = coded || rows > few_rows(dim);
-    c.tile_rows = !many ? (rows > 16 ? 32 : 16) : rows > 128 ? many_rows(dim, coded) : 128;
+    c.tile_rows = !many ? (rows > 16 ? 32 : 16) : many_rows(dim, coded);
+    // 256 rows where they are not a tenth more than tiles of 128 would have (300
+    // rows, 8 x 4 over 16,000 tokens of 128 channels: 118 us in three tiles of
+    // 128, 136 in two of 256; full tiles are a tenth faster with 256)
+    auto padded_rows = [&](int64_t tile) { return (rows + tile - 1) / tile * tile; };
+    if (c.tile_rows == 256 && 10 * padded_rows(256) > 11 * padded_rows(128)) c.tile_rows = 128;
     c.row_tiles = int((rows + c.tile_rows - 1) / c.tile_rows);
     // Few rows: splits of 512 tokens at least (one sequence of 65,536 tokens, 2
     // heads of 64 channels: 23.6 us, with 256 31.7), where that leaves eight of
@@ -179,9 +184,10 @@ Cut cut_of(const kvexp_hip_ctx *ctx, int64_t rows, int64_t pairs, int max_len, i
     // 77 us, with eight 83, with four 73; but 16 of up to 16,411 with up to five
     // drafts, 4 queries of 96 channels: 54, 56, 64). Many rows: 256 at least (30
     // rows over 4,096 compressed tokens: 25 us, with 512 33), and the workgroups
-    // that are resident.
+    // that are resident: one of 256 rows per CU, one of 128 above head_dim 128
+    // (730 rows over 4,586 tokens of 256 channels: 73 us, for two 93), else two.
     c.min_split = many || max_len <= 4096 ? 256 : 512;
-    const int64_t per_cu = !many ? (c.tile_rows == 32 ? 6 : 8) : c.tile_rows == 256 ? 1 : 2;
+    const int64_t per_cu = !many ? (c.tile_rows == 32 ? 6 : 8) : c.tile_rows == 256 || dim > 128 ? 1 : 2;
     const int64_t target = int64_t(std::max(1, ctx->cu_count)) * per_cu;
     const int64_t base = std::max<int64_t>(1, pairs * c.row_tiles);
     // (many rows: no second round for a few more)
