@@ -162,7 +162,7 @@ struct Cut {
 
 // Rows per (sequence, head) pick the kernel: what a workgroup of the few-row
 // kernel takes (few_rows), or the many-row kernel, whose tiles go through LDS.
-Cut cut_of(const kvexp_hip_ctx *ctx, int64_t rows, int64_t pairs, int max_len, int dim, bool coded) {
+Cut cut_of(const kvexp_hip_ctx *ctx, int64_t rows, int64_t pairs, int max_len, int dim, bool shared, bool coded) {
     Cut c;
     if (rows > INT32_MAX / 2) fail(KVEXP_HIP_UNSUPPORTED, "paged attention: too many query rows");
     const bool many = coded || rows > few_rows(dim);
@@ -185,9 +185,13 @@ Cut cut_of(const kvexp_hip_ctx *ctx, int64_t rows, int64_t pairs, int max_len, i
     // drafts, 4 queries of 96 channels: 54, 56, 64). Many rows: 256 at least (30
     // rows over 4,096 compressed tokens: 25 us, with 512 33), and the workgroups
     // that are resident: one of 256 rows per CU, one of 128 above head_dim 128
-    // (730 rows over 4,586 tokens of 256 channels: 73 us, for two 93), else two.
+    // (730 shared rows over 4,586 tokens of 256 channels: 73 us, for two 93), else
+    // two; of unequal sequences and causal tiles twice that (12 prompts of up to
+    // 3,051 tokens, 248 rows of 8 heads of 128 channels: 49 us, else 74; of 256
+    // channels 120 and 192).
     c.min_split = many || max_len <= 4096 ? 256 : 512;
-    const int64_t per_cu = !many ? (c.tile_rows == 32 ? 6 : 8) : c.tile_rows == 256 || dim > 128 ? 1 : 2;
+    const int64_t resident = c.tile_rows == 256 || dim > 128 ? 1 : 2;
+    const int64_t per_cu = !many ? (c.tile_rows == 32 ? 6 : 8) : shared ? resident : 2 * resident;
     const int64_t target = int64_t(std::max(1, ctx->cu_count)) * per_cu;
     const int64_t base = std::max<int64_t>(1, pairs * c.row_tiles);
     // (many rows: no second round for a few more)
@@ -254,7 +258,7 @@ Call plan_call(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, const kvexp_hip
     if (c.has_shared && shared->xkv != nullptr && shared->xkv->device != ctx->device)
         bad(std::string(who) + ": the prefix is on another device");
     const int64_t rows = int64_t(a.batch.max_new) * a.group;
-    c.cut = cut_of(ctx, rows, int64_t(a.batch.n_seqs) * a.n_kv, max_len, a.dim, false);
+    c.cut = cut_of(ctx, rows, int64_t(a.batch.n_seqs) * a.n_kv, max_len, a.dim, false, false);
     // (the merge: a wave per query row)
     if (threads_of(c.cut, int64_t(a.batch.n_seqs) * a.n_kv) > kThreadsMax ||
         int64_t(a.batch.n_tokens) * n_q_heads > kThreadsMax / 64 - 4)
@@ -276,7 +280,7 @@ Call plan_call(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, const kvexp_hip
         p.direct = 0;
         p.len = shared->n_tokens;
         const bool xkv = shared->xkv != nullptr;
-        c.shared_cut = cut_of(ctx, int64_t(a.batch.n_tokens) * a.group, a.n_kv, p.len, a.dim, xkv);
+        c.shared_cut = cut_of(ctx, int64_t(a.batch.n_tokens) * a.group, a.n_kv, p.len, a.dim, true, xkv);
         if (threads_of(c.shared_cut, a.n_kv) > kThreadsMax)
             fail(KVEXP_HIP_UNSUPPORTED, std::string(who) + ": more query rows than a launch takes");
         p.row_tiles = c.shared_cut.row_tiles;
